@@ -1,0 +1,190 @@
+"""Tensor-level entry points of the 8-bit kernels: products of tokens and weights in 8-bit integers, and a cache of keys
+and values held in 8 bits.  As in ``ops``: arguments are checked, kernels are launched on the current CUDA stream, and
+nothing else stands behind these functions.
+
+A number held in 8 bits is a code in [-127, 127] times a float32 scale: one scale a token (activations), an output channel
+(weights), or a page of tokens and kv head (cache).  A scale is max|x| * (1 / 127) and a code rint(x / scale), 0 where the
+scale is 0, each step rounded once in float32.  A row (of the cache: a block) with an infinity or NaN in it gets the scale
+NaN, and all that is computed from it is NaN.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_float, c_int
+
+import torch
+
+from tokasaurus_b200.kernels.ops import _check, _fn, _libs, _need, _need_cuda, _ptr, _stream, _suffix, check_head_dim
+
+MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
+c_longlong = ctypes.c_longlong
+
+
+def _is_f32(dtype: torch.dtype) -> int:
+    return 1 if _suffix(dtype) == "f32" else 0
+
+
+def _stride0(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _code_rows(rows: int, k: int, device) -> torch.Tensor:
+    """Room for rows of codes, each on a 16-byte boundary."""
+    return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
+
+
+def quantise_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes int8 [M, K] (rows on 16-byte boundaries) and scales float32 [M] of the rows of ``x`` (bfloat16 or float32):
+    a step's tokens, or a weight matrix [out, in] that ``linear_int8`` then takes."""
+    _need_cuda(x)
+    _need(x.dim() == 2 and x.shape[1] >= 1 and (x.stride(1) == 1 or x.shape[1] == 1), "quantise_rows: rows of numbers that lie together")
+    f32 = _is_f32(x.dtype)
+    M, K = x.shape
+    codes = _code_rows(M, K, x.device)
+    scale = torch.empty((M,), dtype=torch.float32, device=x.device)
+    _check(_fn(_libs.get("int8_product.cu"), "tkb_quantise_rows")(
+        _ptr(x), c_longlong(x.stride(0)), c_int(f32), _ptr(codes), c_longlong((K + 15) // 16 * 16), _ptr(scale), c_int(M), c_int(K),
+        _stream()), "quantise_rows")
+    return codes, scale
+
+
+def product_int8(codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status: torch.Tensor,
+                 gated: bool = False, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(codes @ w^T) * scale[:, None] * w_scale`` of 8-bit codes [M, K] and [N, K] (rows on 16-byte boundaries); the sums
+    are exact.  ``gated``: ``w`` and ``w_scale`` interleave gate and up rows (``ops.interleave_gate_up``), the result is
+    silu(gate) * up [M, N / 2]."""
+    _need_cuda(codes, scale, w, w_scale, status)
+    _need(codes.dtype == torch.int8 and w.dtype == torch.int8 and codes.dim() == 2 and w.dim() == 2 and codes.shape[1] == w.shape[1],
+          "product_int8: int8 codes [M, K] and [N, K]")
+    M, K = codes.shape
+    N = w.shape[0]
+    _need(1 <= K <= MAX_K and N >= 1, f"product_int8: 1 to {MAX_K} numbers a row (their sum has to fit 32 bits)")
+    for t, what in ((codes, "tokens"), (w, "weights")):
+        _need((t.stride(1) == 1 or K == 1) and (t.shape[0] <= 1 or t.stride(0) % 16 == 0) and t.data_ptr() % 16 == 0,
+              f"product_int8: rows of the {what}' codes lie on 16-byte boundaries (quantise_rows and lay_out_codes leave them so)")
+    _need(scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == M, "product_int8: token scales float32 [M]")
+    _need(w_scale.dtype == torch.float32 and w_scale.is_contiguous() and w_scale.numel() == N, "product_int8: channel scales float32 [N]")
+    _need(not gated or N % 16 == 0, "product_int8: gated weights come in groups of 16 rows")
+    out = torch.empty((M, N // 2 if gated else N), dtype=out_dtype, device=codes.device)
+    _check(_fn(_libs.get("int8_product.cu"), "tkb_int8_product")(
+        _ptr(codes), c_longlong(codes.stride(0)), _ptr(scale), _ptr(w), c_longlong(w.stride(0)), _ptr(w_scale), _ptr(out),
+        c_longlong(out.shape[1]), c_int(_is_f32(out_dtype)), c_int(M), c_int(N), c_int(K), c_int(1 if gated else 0), _ptr(status),
+        _stream()), "product_int8")
+    return out
+
+
+def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status: torch.Tensor, gated: bool = False,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ (w * w_scale[:, None])^T`` with ``x`` [M, K] (bfloat16 or float32) brought to 8 bits token by token and the
+    products summed in integers.  The result has ``out_dtype`` (``x``'s if None)."""
+    codes, scale = quantise_rows(x)
+    return product_int8(codes, scale, w, w_scale, status, gated, out_dtype or x.dtype)
+
+
+def lay_out_codes(w: torch.Tensor) -> torch.Tensor:
+    """A copy of int8 codes [N, K] whose rows lie on 16-byte boundaries, as ``product_int8`` asks."""
+    _need(w.dtype == torch.int8 and w.dim() == 2, "lay_out_codes: int8 [N, K]")
+    out = _code_rows(w.shape[0], w.shape[1], w.device)
+    out.copy_(w)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+def _check_cache(what: str, kcache, vcache, k_scale, v_scale, n_kv_heads: int, page_size: int, head_dim: int) -> None:
+    for c, s in ((kcache, k_scale), (vcache, v_scale)):
+        _need(c.dtype == torch.int8 and c.is_contiguous() and c.dim() == 4 and tuple(c.shape[1:]) == (n_kv_heads, page_size, head_dim),
+              f"{what}: the cache is int8 [pages, kv heads, page size, head size]")
+        _need(s.dtype == torch.float32 and s.is_contiguous() and tuple(s.shape) == tuple(c.shape[:2]), f"{what}: scales are float32 [pages, kv heads]")
+        _need(c.data_ptr() % 16 == 0, f"{what}: the cache starts on a 16-byte boundary")
+    _need(kcache.shape[0] == vcache.shape[0], f"{what}: as many pages of keys as of values")
+
+
+def _need_i32(what: str, **tensors) -> None:
+    for name, t in tensors.items():
+        _need(t.dtype == torch.int32 and t.is_contiguous(), f"{what}: {name} is int32, contiguous")
+
+
+def rope_kv8_write(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, page_indptr: torch.Tensor,
+                   page_ids: torch.Tensor, inv_freq: torch.Tensor | None, kcache: torch.Tensor, vcache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, rotary_dim: int,
+                   page_size: int, write_cache: bool, status: torch.Tensor) -> None:
+    """``ops.rope_kv_write`` for a cache held in 8 bits: rotate q (in place) and k by position, write k and v as codes under
+    one scale a page and kv head.  kcache/vcache: int8 [pages, n_kv_heads, page_size, head_dim]; k_scale/v_scale: float32
+    [pages, n_kv_heads].
+
+    A block's scale only grows while its page is filled: when new numbers top it, the codes that the page holds are brought
+    to the larger scale.  A token in a page's first slot starts the page afresh.  Tokens of one request stand together, in
+    the order of their positions; one request's page is written by its own tokens only."""
+    what = "rope_kv8_write"
+    _need_cuda(qkv, positions, token_seq, page_indptr, page_ids, inv_freq, kcache, vcache, k_scale, v_scale, status)
+    f32 = _is_f32(qkv.dtype)
+    n = qkv.shape[0]
+    _need(n_heads >= 1 and n_kv_heads >= 1 and page_size >= 1, f"{what}: sizes")
+    check_head_dim(head_dim)
+    _need(qkv.dim() == 2 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim, f"{what}: qkv shape")
+    _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    _need_i32(what, positions=positions, token_seq=token_seq, page_indptr=page_indptr, page_ids=page_ids)
+    _need(positions.numel() >= n and token_seq.numel() >= n, f"{what}: a position and a request a token")
+    _need(0 <= rotary_dim <= head_dim and rotary_dim % 2 == 0, f"{what}: rotary_dim")
+    if rotary_dim:
+        _need(inv_freq is not None and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.numel() == rotary_dim // 2,
+              f"{what}: inv_freq must be float32 [rotary_dim/2]")
+    _check(_fn(_libs.get("cache8.cu"), "tkb_rope_kv8_write")(
+        _ptr(qkv), c_int(f32), _ptr(positions), _ptr(token_seq), _ptr(page_indptr), _ptr(page_ids), _ptr(inv_freq), _ptr(kcache),
+        _ptr(vcache), _ptr(k_scale), _ptr(v_scale), c_int(n), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(rotary_dim),
+        c_int(page_size), c_int(kcache.shape[0]), c_int(1 if write_cache else 0), _ptr(status), _stream()), what)
+
+
+def read_kv8(kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, pages: torch.Tensor,
+             status: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that ``pages`` (int32 [n]) hold, as float32 [n, kv heads, page size, head size] each; zeros for an
+    id that is negative or beyond the pool (the latter sets the status word's page bit)."""
+    _need_cuda(kcache, vcache, k_scale, v_scale, pages, status)
+    _need(kcache.dim() == 4, "read_kv8: the cache is int8 [pages, kv heads, page size, head size]")
+    n_kv, ps, hd = kcache.shape[1:]
+    _check_cache("read_kv8", kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
+    _need_i32("read_kv8", pages=pages)
+    _need(ps * hd % 16 == 0, "read_kv8: page size times head size is a multiple of 16")
+    n = pages.numel()
+    k = torch.empty((n, n_kv, ps, hd), dtype=torch.float32, device=kcache.device)
+    v = torch.empty_like(k)
+    _check(_fn(_libs.get("cache8.cu"), "tkb_read_kv8")(
+        _ptr(kcache), _ptr(vcache), _ptr(k_scale), _ptr(v_scale), _ptr(pages), _ptr(k), _ptr(v), c_int(n), c_int(n_kv), c_int(ps * hd),
+        c_int(kcache.shape[0]), _ptr(status), _stream()), "read_kv8")
+    return k, v
+
+
+def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+             q_start: torch.Tensor, q_len: torch.Tensor, kv_len: torch.Tensor, page_indptr: torch.Tensor, page_ids: torch.Tensor,
+             n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float, window: int | None, status: torch.Tensor,
+             max_q_len: int, max_kv_len: int, single_tokens: int) -> None:
+    """Causal grouped-query attention of a step's tokens over a cache held in 8 bits.
+
+    q: rotated queries, the first n_heads*head_dim columns of rows [T, >= that] (bfloat16 or float32); out: [T, n_heads*head_dim]
+    of q's type.  Request s brings the q_len[s] tokens from row q_start[s] on, the last of its kv_len[s] keys, which its pages
+    (``page_ids`` from ``page_indptr[s]`` on) hold; the tokens must have been written before.  A token sees the keys up to its own
+    position, with ``window`` only the last so many, none on pages given back (id -1); one that sees none gets 0.
+
+    Bounds known to the host, from which the launch is sized: ``max_q_len`` and ``max_kv_len`` over all requests,
+    ``single_tokens``: how many requests bring one token (requests beyond these bounds are not computed whole)."""
+    what = "attn_kv8"
+    _need_cuda(q, out, kcache, vcache, k_scale, v_scale, q_start, q_len, kv_len, page_indptr, page_ids, status)
+    f32 = _is_f32(q.dtype)
+    check_head_dim(head_dim)
+    _need(n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0 and page_size >= 1, f"{what}: heads in groups of a kv head")
+    width = n_heads * head_dim
+    for t, name in ((q, "q"), (out, "out")):
+        _need(t.dim() == 2 and t.shape[1] >= width and t.stride(1) == 1 and t.dtype == q.dtype, f"{what}: {name} has rows of heads of one type")
+    _need(out.shape[0] >= q.shape[0], f"{what}: a row of out for every row of q")
+    _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    _need_i32(what, q_start=q_start, q_len=q_len, kv_len=kv_len, page_indptr=page_indptr, page_ids=page_ids)
+    n = q_len.numel()
+    _need(q_start.numel() >= n and kv_len.numel() >= n and page_indptr.numel() > n, f"{what}: a start, a length and pages for every request")
+    _need(window is None or window >= 1, f"{what}: a window of one key at least")
+    _need(max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n, f"{what}: bounds")
+    _check(_fn(_libs.get("attention_kv8.cu"), "tkb_attn_kv8")(
+        _ptr(q), c_longlong(_stride0(q)), _ptr(out), c_longlong(_stride0(out)), c_int(f32), _ptr(kcache), _ptr(vcache), _ptr(k_scale),
+        _ptr(v_scale), _ptr(q_start), _ptr(q_len), _ptr(kv_len), _ptr(page_indptr), _ptr(page_ids), c_int(n), c_int(max_q_len),
+        c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(page_size), c_float(scale), c_int(window or 0), c_int(kcache.shape[0]),
+        _ptr(status), _stream()), what)

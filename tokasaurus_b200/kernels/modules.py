@@ -47,6 +47,11 @@ def family_modules() -> list[tuple[str, dict | None]]:
             ("attention_rows_tc.cu", {"TKB_ROW": 256, "TKB_KD": 128, "TKB_V0": 128, "TKB_VD": 128, "TKB_CAP": 1})]
 
 
+def int8_modules(head_dims=()) -> list[tuple[str, dict | None]]:
+    """Products in 8-bit integers, and the cache held in 8 bits with the attention over it."""
+    return [("int8_product.cu", None), ("cache8.cu", None), ("attention_kv8.cu", None)]
+
+
 def optional_modules(head_dim: int) -> list[tuple[str, dict | None]]:
     """Built by the build check, loaded only by callers that ask for them."""
     return EXTRA + [("attention_decode_static.cu", {"TKB_HD": head_dim})]
