@@ -4,10 +4,16 @@
 //     s = max_k |x| * (1 / 127),   c = rint(x / s) held to [-127, 127], 0 where s is 0,
 // each step rounded once in float32, so that the codes do not depend on how the work is cut.  A row with an infinity or
 // NaN gets the scale NaN and the codes 0: its results are NaN, those of other rows are not touched.
-// w, t: an output channel's codes and scale.  The sum is a 32-bit integer, exact for K up to 132,103 (127 * 128 * K < 2^31).
-#include "common.cuh"
+// w, t: an output channel's codes and scale.  The sum is a 32-bit integer, exact for K up to 132,103 (127 * 128 * K < 2^31):
+// however K is cut and in whichever order its parts are added, a token's result has the same bits.
+//
+// Both products run on the fifth-generation tensor cores (tcgen05.mma kind::i8, 32-bit integer accumulators in tensor
+// memory), fed by TMA in boxes of 128 codes (one 128-byte swizzle row) a row.  Every wait on an mbarrier is bounded: after
+// the limit the block sets TKB_STATUS_WAIT_TIMEOUT, stops waiting, frees its tensor memory and returns.
+#include "tcgen05.cuh"
+#include "per_device.h"
 
-using namespace tkb;
+using namespace tkb5;
 
 namespace {
 
@@ -29,8 +35,10 @@ __global__ void __launch_bounds__(Q_THREADS)
 quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc, float* __restrict__ scale,
                      int K) {
   __shared__ unsigned s_top[Q_THREADS / 32];
-  trigger_dependents();
+  // The product behind this kernel may fetch weights as soon as it has started: only then, when every kernel ahead of this
+  // one (one that made those weights among them) is over.
   grid_dependency_wait();
+  trigger_dependents();
   const T* row = x + (long long)blockIdx.x * ldx;
   int8_t* dst = codes + (long long)blockIdx.x * ldc;
   // magnitudes as integers: NaN > infinity > every number
@@ -49,59 +57,442 @@ quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
 
-// 64 tokens x 64 channels a block, 32 codes of K at a time through shared memory, four by four results a thread.
-constexpr int TILE = 64, KSTEP = 32;
+// ------------------------------------------------------------------------------------------------ shared by both products
+constexpr int BK8 = 128;    // codes of K a box: one swizzle row
+constexpr int THREADS = 192;
 
-template <typename T>
-__global__ void __launch_bounds__(256)
-product_kernel(const int8_t* __restrict__ a, long long lda, const float* __restrict__ a_scale, const int8_t* __restrict__ w,
-               long long ldw, const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int M, int N, int K, int gated) {
-  __shared__ int sa[TILE][KSTEP / 4 + 1], sw[TILE][KSTEP / 4 + 1];
-  __shared__ float tile[TILE][TILE + 1];
+// Instruction descriptor: D = 32-bit integers, A = B = signed 8-bit, both K-major, shape M x N.
+__host__ __device__ constexpr uint32_t make_idesc8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Four instructions (32 codes of K each) on one 128-code box of A and of B.
+__device__ __forceinline__ void umma8_box(uint32_t tmem_d, uint32_t a_addr, uint32_t b_addr, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int k = 0; k < 4; k++) umma8(tmem_d, make_desc(a_addr + k * 32), make_desc(b_addr + k * 32), idesc, (!first || k > 0) ? 1u : 0u);
+}
+static int make_map8(CUtensorMap* map, const void* base, long long rows, int K, long long ld, int box_rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)BK8, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
+}
+__device__ __forceinline__ float value_of(uint32_t sum, float st) { return (float)(int)sum * st; }
+
+__device__ __forceinline__ void store8(bf16* dst, const float (&y)[8], bool whole, int left) {
+  if (whole && (((uintptr_t)dst) & 15) == 0) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < left) dst[i] = __float2bfloat16_rn(y[i]);
+  }
+}
+__device__ __forceinline__ void store8(float* dst, const float (&y)[8], bool whole, int left) {
+  if (whole && (((uintptr_t)dst) & 15) == 0) {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(y[0], y[1], y[2], y[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(y[4], y[5], y[6], y[7]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (i < left) dst[i] = y[i];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ many tokens
+// A block computes 128-token x BN-channel tiles, one after the other (persistent).  Warp 0: one lane issues the TMA loads into a
+// ring of stages; warp 1: tensor memory, one lane issues the MMAs; warps 2-5: a tile's accumulator from tensor memory, scaled
+// (gated: silu(gate) * up) and stored while the next tile's MMAs fill the other accumulator.
+constexpr int BM = 128;
+
+template <int BN> struct Cfg {
+  static constexpr int A_BYTES = BM * BK8;  // 16 KiB
+  static constexpr int STAGE_BYTES = A_BYTES + BN * BK8;
+  static constexpr int STAGES = BN >= 256 ? 4 : 6;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  static constexpr int TMEM_COLS = 2 * BN;
+};
+
+template <int BN, bool GATED, typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+product_many_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const float* __restrict__ a_scale,
+                    const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int M, int N, int K, int* __restrict__ status) {
+  extern __shared__ unsigned char smem_raw[];
+  constexpr int STAGES = Cfg<BN>::STAGES;
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(16) float col_scale[2][BN];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int failed;
+  unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_kblocks = (K + BK8 - 1) / BK8;
+  const int m_tiles = (M + BM - 1) / BM, n_tiles = (N + BN - 1) / BN;
+  const int total_tiles = m_tiles * n_tiles;
   trigger_dependents();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);  // one arrival from each epilogue warp
+    }
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // Tensor memory is taken only after the kernel ahead has finished: a block of that kernel that still waits for columns on
+  // this SM could otherwise wait for this block, which waits for that kernel.
   grid_dependency_wait();
-  const int m0 = blockIdx.y * TILE, n0 = blockIdx.x * TILE;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += KSTEP) {
-    for (int i = threadIdx.x; i < TILE * KSTEP / 4; i += 256) {
-      const int r = i / (KSTEP / 4), c = i % (KSTEP / 4), k = k0 + 4 * c;
-      int va = 0, vw = 0;
-      for (int e = 0; e < 4; e++)
-        if (k + e < K) {
-          if (m0 + r < M) va |= (int)(uint8_t)a[(m0 + r) * lda + k + e] << (8 * e);
-          if (n0 + r < N) vw |= (int)(uint8_t)w[(n0 + r) * ldw + k + e] << (8 * e);
-        }
-      sa[r][c] = va;
-      sw[r][c] = vw;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < KSTEP / 4; c++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = __dp4a(sa[ty + 16 * i][c], sw[tx + 16 * j][c], acc[i][j]);
-    __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
+                 "r"((uint32_t)Cfg<BN>::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N) tile[ty + 16 * i][tx + 16 * j] = (float)acc[i][j] * (a_scale[m] * w_scale[n]);
-    }
+  tcgen05_fence_before();
   __syncthreads();
-  for (int i = threadIdx.x; i < TILE * TILE; i += 256) {
-    const int r = i / TILE, c = i % TILE, m = m0 + r, n = n0 + c;
-    if (m >= M || n >= N) continue;
-    if (!gated) {
-      out[m * ldo + n] = from_float<T>(tile[r][c]);
-    } else if ((c & 8) == 0) {
-      const float g = tile[r][c], u = tile[r][c + 8];
-      out[m * ldo + (n >> 4) * 8 + (c & 7)] = from_float<T>(g / (1.f + expf(-g)) * u);
+  tcgen05_fence_after();
+  const uint32_t tmem_acc = tmem_base_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+        const int m0 = (t % m_tiles) * BM, n0 = (t / m_tiles) * BN;
+        for (int kb = 0; kb < n_kblocks; kb++, it++) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !mbar_wait(&empty_bar[s], ((it / STAGES) - 1) & 1)) { failed = 1; ok = false; break; }
+          unsigned char* dst = ring + s * Cfg<BN>::STAGE_BYTES;
+          mbar_expect_tx(&full_bar[s], Cfg<BN>::STAGE_BYTES);
+          tma_load_2d(dst, &map_a, &full_bar[s], kb * BK8, m0);
+          tma_load_2d(dst + Cfg<BN>::A_BYTES, &map_w, &full_bar[s], kb * BK8, n0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc8(BM, BN);
+      uint32_t it = 0, j = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x, j++) {
+        const uint32_t buf = j & 1;
+        if (j >= 2 && !mbar_wait(&acc_empty[buf], ((j >> 1) - 1) & 1)) { failed = 1; break; }
+        tcgen05_fence_after();
+        for (int kb = 0; kb < n_kblocks; kb++, it++) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&full_bar[s], (it / STAGES) & 1)) { failed = 1; ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t a_addr = smem_u32(ring + s * Cfg<BN>::STAGE_BYTES);
+          umma8_box(tmem_acc + buf * BN, a_addr, a_addr + Cfg<BN>::A_BYTES, idesc, kb == 0);
+          tcgen05_commit(&empty_bar[s]);
+        }
+        tcgen05_commit(&acc_full[buf]);
+      }
+    }
+  } else {
+    const int q = warp & 3;  // the quarter of tensor memory that this warp may touch
+    uint32_t j = 0;
+    bool ok = true;  // (a warp whose wait ran out goes on to the others' barriers)
+    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, j++) {
+      const uint32_t buf = j & 1;
+      const int m0 = (t % m_tiles) * BM, n0 = (t / m_tiles) * BN;
+      // the tile's channel scales (the other buffer is still read by slower warps)
+      for (int i = threadIdx.x - 64; i < BN; i += 128) col_scale[buf][i] = n0 + i < N ? w_scale[n0 + i] : 0.f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ok = ok && mbar_wait(&acc_full[buf], (j >> 1) & 1);
+      if (!ok) { failed = 1; continue; }
+      tcgen05_fence_after();
+      const int row = m0 + q * 32 + lane;
+      const float rs = row < M ? a_scale[row] : 0.f;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        if (n0 + c0 >= N) break;
+        uint32_t r[32];
+        tmem_ld32(tmem_acc + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + c0), r);
+        if (row < M) {
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 cs = *reinterpret_cast<const float4*>(&col_scale[buf][c0 + i]);
+            y[i] = value_of(r[i], rs * cs.x), y[i + 1] = value_of(r[i + 1], rs * cs.y);
+            y[i + 2] = value_of(r[i + 2], rs * cs.z), y[i + 3] = value_of(r[i + 3], rs * cs.w);
+          }
+          const int n = n0 + c0;
+          if (!GATED) {
+            T* dst = out + (long long)row * ldo + n;
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+              float z[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) z[i] = y[8 * v + i];
+              store8(dst + 8 * v, z, n + 8 * v + 8 <= N, N - n - 8 * v);
+            }
+          } else {
+            // columns come in groups of 16: 8 gate columns, then the 8 up columns of the same features
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+              float z[8];
+#pragma unroll
+              for (int i = 0; i < 8; i++) z[i] = silu_mul_fast(y[16 * g + i], y[16 * g + 8 + i]);
+              if (n + 16 * g + 16 <= N) store8(out + (long long)row * ldo + (n >> 1) + 8 * g, z, true, 8);
+            }
+          }
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+    tcgen05_fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"((uint32_t)Cfg<BN>::TMEM_COLS) : "memory");
+  }
+  if (threadIdx.x == 0 && failed) atomicOr(status, TKB_STATUS_WAIT_TIMEOUT);
+}
+
+template <int BN, bool GATED, typename T>
+int launch_many(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
+                long long ldo, int M, int N, int K, int weights_ready, int* status, cudaStream_t st) {
+  static SharedMemoryRequest ask;
+  int rc = ask({{(const void*)product_many_kernel<BN, GATED, T>, Cfg<BN>::SMEM_BYTES}});
+  if (rc) return rc;
+  CUtensorMap map_a, map_w;
+  if ((rc = make_map8(&map_a, a, M, K, lda, BM)) || (rc = make_map8(&map_w, w, N, K, ldw, BN))) return rc;
+  const int n_sms = sm_count();
+  const long long tiles = (long long)((N + BN - 1) / BN) * ((M + BM - 1) / BM);
+  if (tiles > 2147483647ll) return -3;
+  return launch_pdl(product_many_kernel<BN, GATED, T>, dim3(tiles < n_sms ? (int)tiles : n_sms), dim3(THREADS), (size_t)Cfg<BN>::SMEM_BYTES,
+                    st, map_a, map_w, a_scale, w_scale, (T*)out, ldo, M, N, K, status);
+}
+
+// ------------------------------------------------------------------------------------------------ few tokens
+// The CHANNELS are the 128-row side of the instruction and the tokens its 16 to 128 columns, so that the weights stream at memory
+// speed whatever the token count.  A block owns 128 channels and one part of K; the parts of one tile form a CLUSTER, whose
+// blocks hand their 32-bit sums to one another through shared memory (each sums the tokens that are its own, in integers:
+// the order does not matter), scale them and store them.  With programmatic dependent launch the weights of the first stages
+// are on their way while the tokens are still being brought to codes.
+constexpr int BC = 128;                // channels a block
+constexpr int W8_BYTES = BC * BK8;     // 16 KiB
+
+template <int NTOK> struct FewCfg {
+  static constexpr int STAGE_BYTES = W8_BYTES + NTOK * BK8;
+  static constexpr int STAGES = NTOK >= 128 ? 3 : NTOK >= 64 ? 4 : 5;  // two blocks an SM
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
+  static constexpr int TMEM_COLS = NTOK < 32 ? 32 : NTOK;
+};
+constexpr int MAX_PARTS = 8;
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void store_remote(uint32_t addr, int rank, uint32_t v) {
+  asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nst.shared::cluster.u32 [r], %2;\n}" ::"r"(addr), "r"(rank), "r"(v) : "memory");
+}
+
+template <int NTOK, bool GATED, typename T>
+__global__ void __launch_bounds__(THREADS, 2)
+product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ a_scale,
+                   const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int M, int N, int K, int kblocks_per_part,
+                   int weights_ready, int* __restrict__ status) {
+  extern __shared__ unsigned char smem_raw[];
+  constexpr int STAGES = FewCfg<NTOK>::STAGES, STAGE_BYTES = FewCfg<NTOK>::STAGE_BYTES, TMEM_COLS = FewCfg<NTOK>::TMEM_COLS;
+  __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int failed;
+  unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * BC;
+  const int part = blockIdx.y, parts = gridDim.y;  // a cluster is all parts of a tile
+  const int kb_begin = part * kblocks_per_part;
+  const int nkb = max(0, min(kblocks_per_part, (K + BK8 - 1) / BK8 - kb_begin));
+
+  trigger_dependents();
+  const int first = nkb < STAGES ? nkb : STAGES;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(&acc_bar, 1);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // With `weights_ready` nothing that may still be running writes the weights: they are asked for before the tokens' codes exist.
+    if (!weights_ready) grid_dependency_wait();
+    for (int kb = 0; kb < first; kb++) {
+      mbar_expect_tx(&full_bar[kb], STAGE_BYTES);
+      tma_load_2d(ring + kb * STAGE_BYTES, &map_w, &full_bar[kb], (kb_begin + kb) * BK8, n0);
     }
   }
+  if (warp == 1) {
+    grid_dependency_wait();  // (before tensor memory is taken, as in the kernel above)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
+                 "r"((uint32_t)TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_acc = tmem_base_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      grid_dependency_wait();
+      for (int kb = 0; kb < first; kb++)
+        tma_load_2d(ring + kb * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[kb], (kb_begin + kb) * BK8, 0);
+      for (int kb = STAGES; kb < nkb; kb++) {
+        const int s = kb % STAGES;
+        if (!mbar_wait(&empty_bar[s], ((kb / STAGES) - 1) & 1)) { failed = 1; break; }
+        mbar_expect_tx(&full_bar[s], STAGE_BYTES);
+        tma_load_2d(ring + s * STAGE_BYTES, &map_w, &full_bar[s], (kb_begin + kb) * BK8, n0);
+        tma_load_2d(ring + s * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[s], (kb_begin + kb) * BK8, 0);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc8(BC, NTOK);
+      for (int kb = 0; kb < nkb; kb++) {
+        const int s = kb % STAGES;
+        if (!mbar_wait(&full_bar[s], (kb / STAGES) & 1)) { failed = 1; break; }
+        tcgen05_fence_after();
+        const uint32_t w_addr = smem_u32(ring + s * STAGE_BYTES);
+        umma8_box(tmem_acc, w_addr, w_addr + W8_BYTES, idesc, kb == 0);
+        tcgen05_commit(&empty_bar[s]);
+      }
+      tcgen05_commit(&acc_bar);
+    }
+  }
+  __syncwarp();
+  const int q = warp & 3, f = q * 32 + lane;  // an epilogue thread's channel of the block's
+  const uint32_t t_addr = tmem_acc + ((uint32_t)(q * 32) << 16);
+  bool ok = true;
+  if (warp >= 2) {
+    grid_dependency_wait();  // nothing is stored before the kernel ahead of this one has finished
+    ok = mbar_wait(&acc_bar, 0);
+    tcgen05_fence_after();
+    if (!ok) failed = 1;
+  }
+  const float ts = warp >= 2 && n0 + f < N ? w_scale[n0 + f] : 0.f;
+  auto finish = [&](int m, uint32_t sum) {
+    // one token's sum of this thread's channel: scaled and stored (gated: the up channel's value comes from eight lanes on)
+    const float y = value_of(sum, a_scale[m] * ts);
+    if (!GATED) {
+      if (n0 + f < N) out[(long long)m * ldo + n0 + f] = from_float<T>(y);
+    } else {
+      const float up = __shfl_down_sync(0xffffffffu, y, 8);
+      if ((lane & 8) == 0 && n0 + f + 8 < N) out[(long long)m * ldo + ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7)] = from_float<T>(silu_mul_fast(y, up));
+    }
+  };
+  if (parts == 1) {
+    if (warp >= 2 && ok) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < NTOK && c0 < M; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(t_addr + c0, r);
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (c0 + i < M) finish(c0 + i, r[i]);
+      }
+    }
+  } else {
+    // token c belongs to part c % parts; its sums stand there as [c / parts][part][channel], where the ring was
+    uint32_t* sums = reinterpret_cast<uint32_t*>(ring);
+    cluster_sync();  // every block's MMAs have read their stages
+    if (warp >= 2 && ok) {
+#pragma unroll 1
+      for (int c0 = 0; c0 < NTOK && c0 < M; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(t_addr + c0, r);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int c = c0 + i;
+          if (c < M) store_remote(smem_u32(&sums[((c / parts) * parts + part) * BC + f]), c % parts, r[i]);
+        }
+      }
+    }
+    cluster_sync();
+    if (warp >= 2) {
+      for (int c = part; c < M; c += parts) {
+        uint32_t sum = 0;
+        for (int i = 0; i < parts; i++) sum += sums[((c / parts) * parts + i) * BC + f];
+        finish(c, sum);
+      }
+    }
+  }
+  if (warp >= 2) tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"((uint32_t)TMEM_COLS) : "memory");
+  }
+  if (threadIdx.x == 0 && failed) atomicOr(status, TKB_STATUS_WAIT_TIMEOUT);
+}
+
+template <int NTOK, bool GATED, typename T>
+int launch_few(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
+               long long ldo, int M, int N, int K, int weights_ready, int* status, cudaStream_t st) {
+  static SharedMemoryRequest ask;
+  constexpr int SMEM = FewCfg<NTOK>::SMEM_BYTES;
+  int rc = ask({{(const void*)product_few_kernel<NTOK, GATED, T>, SMEM}});
+  if (rc) return rc;
+  CUtensorMap map_a, map_w;
+  if ((rc = make_map8(&map_w, w, N, K, ldw, BC)) || (rc = make_map8(&map_a, a, M, K, lda, NTOK))) return rc;
+  const int tiles = (N + BC - 1) / BC, kblocks = (K + BK8 - 1) / BK8;
+  int parts = sm_count() / tiles;
+  if (parts > MAX_PARTS) parts = MAX_PARTS;
+  if (parts > kblocks / 2) parts = kblocks / 2;
+  if (parts < 1) parts = 1;
+  const int per = (kblocks + parts - 1) / parts;
+  parts = (kblocks + per - 1) / per;
+  static_assert((NTOK + MAX_PARTS) * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles, parts);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = parts;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, product_few_kernel<NTOK, GATED, T>, map_w, map_a, a_scale, w_scale, (T*)out, ldo, M, N, K, per, weights_ready, status);
+}
+
+template <bool GATED, typename T>
+int product(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
+            long long ldo, int M, int N, int K, int weights_ready, int* status, cudaStream_t st) {
+#define TKB_ARGS a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st
+  if (M <= 16) return launch_few<16, GATED, T>(TKB_ARGS);
+  if (M <= 32) return launch_few<32, GATED, T>(TKB_ARGS);
+  if (M <= 64) return launch_few<64, GATED, T>(TKB_ARGS);
+  if (M <= 128) return launch_few<128, GATED, T>(TKB_ARGS);
+  if (N >= 256) return launch_many<256, GATED, T>(TKB_ARGS);
+  return launch_many<128, GATED, T>(TKB_ARGS);
+#undef TKB_ARGS
 }
 
 }  // namespace
@@ -113,20 +504,22 @@ TKB_EXPORT int tkb_quantise_rows(const void* x, long long ldx, int f32, void* co
   cudaStream_t st = (cudaStream_t)st_;
   if (f32)
     return launch_pdl(quantise_rows_kernel<float>, dim3(M), dim3(Q_THREADS), 0, st, (const float*)x, ldx, (int8_t*)codes, ldc, (float*)scale, K);
-  return launch_pdl(quantise_rows_kernel<__nv_bfloat16>, dim3(M), dim3(Q_THREADS), 0, st, (const __nv_bfloat16*)x, ldx, (int8_t*)codes, ldc, (float*)scale, K);
+  return launch_pdl(quantise_rows_kernel<bf16>, dim3(M), dim3(Q_THREADS), 0, st, (const bf16*)x, ldx, (int8_t*)codes, ldc, (float*)scale, K);
 }
 
 // out [M, N] (gated: [M, N / 2], rows of w interleaving gate and up in eights) float32 or bfloat16, row stride ldo elements.
-TKB_EXPORT int tkb_int8_product(const void* a, long long lda, const void* a_scale, const void* w, long long ldw, const void* w_scale,
-                                void* out, long long ldo, int f32, int M, int N, int K, int gated, int* status, void* st_) {
+// a, w: codes whose rows start on 16-byte boundaries (row strides lda, ldw in bytes).  weights_ready: the kernel ahead in the
+// stream is tkb_quantise_rows (of the tokens), so that no kernel that may still be running writes w.
+TKB_EXPORT int tkb_int8_product(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale,
+                                void* out, long long ldo, int f32, int M, int N, int K, int gated, int weights_ready, int* status, void* st_) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K > 132103 || (gated && (N & 15))) return -2;
-  if ((M + TILE - 1) / TILE > 65535) return -3;
+  if (K <= 0 || K > 132103 || (gated && (N & 15)) || (lda & 15) || (ldw & 15) || (((uintptr_t)a) & 15) || (((uintptr_t)w) & 15)) return -2;
+  int rc = get_encode();
+  if (rc) return rc;
   cudaStream_t st = (cudaStream_t)st_;
-  const dim3 grid((N + TILE - 1) / TILE, (M + TILE - 1) / TILE);
-  if (f32)
-    return launch_pdl(product_kernel<float>, grid, dim3(256), 0, st, (const int8_t*)a, lda, (const float*)a_scale, (const int8_t*)w, ldw,
-                      (const float*)w_scale, (float*)out, ldo, M, N, K, gated);
-  return launch_pdl(product_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, (const int8_t*)a, lda, (const float*)a_scale, (const int8_t*)w, ldw,
-                    (const float*)w_scale, (__nv_bfloat16*)out, ldo, M, N, K, gated);
+  if (gated)
+    return f32 ? product<true, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
+               : product<true, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
+  return f32 ? product<false, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
+             : product<false, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
 }

@@ -29,6 +29,10 @@ def _stride0(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _code_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
 def _code_rows(rows: int, k: int, device) -> torch.Tensor:
     """Room for rows of codes, each on a 16-byte boundary."""
     return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
@@ -54,6 +58,10 @@ def product_int8(codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_sc
     """``(codes @ w^T) * scale[:, None] * w_scale`` of 8-bit codes [M, K] and [N, K] (rows on 16-byte boundaries); the sums
     are exact.  ``gated``: ``w`` and ``w_scale`` interleave gate and up rows (``ops.interleave_gate_up``), the result is
     silu(gate) * up [M, N / 2]."""
+    return _product(codes, scale, w, w_scale, status, gated, out_dtype, 0)
+
+
+def _product(codes, scale, w, w_scale, status, gated, out_dtype, weights_ready: int) -> torch.Tensor:
     _need_cuda(codes, scale, w, w_scale, status)
     _need(codes.dtype == torch.int8 and w.dtype == torch.int8 and codes.dim() == 2 and w.dim() == 2 and codes.shape[1] == w.shape[1],
           "product_int8: int8 codes [M, K] and [N, K]")
@@ -68,9 +76,9 @@ def product_int8(codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_sc
     _need(not gated or N % 16 == 0, "product_int8: gated weights come in groups of 16 rows")
     out = torch.empty((M, N // 2 if gated else N), dtype=out_dtype, device=codes.device)
     _check(_fn(_libs.get("int8_product.cu"), "tkb_int8_product")(
-        _ptr(codes), c_longlong(codes.stride(0)), _ptr(scale), _ptr(w), c_longlong(w.stride(0)), _ptr(w_scale), _ptr(out),
-        c_longlong(out.shape[1]), c_int(_is_f32(out_dtype)), c_int(M), c_int(N), c_int(K), c_int(1 if gated else 0), _ptr(status),
-        _stream()), "product_int8")
+        _ptr(codes), c_longlong(_code_stride(codes)), _ptr(scale), _ptr(w), c_longlong(_code_stride(w)), _ptr(w_scale), _ptr(out),
+        c_longlong(out.shape[1]), c_int(_is_f32(out_dtype)), c_int(M), c_int(N), c_int(K), c_int(1 if gated else 0), c_int(weights_ready),
+        _ptr(status), _stream()), "product_int8")
     return out
 
 
@@ -79,7 +87,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status:
     """``x @ (w * w_scale[:, None])^T`` with ``x`` [M, K] (bfloat16 or float32) brought to 8 bits token by token and the
     products summed in integers.  The result has ``out_dtype`` (``x``'s if None)."""
     codes, scale = quantise_rows(x)
-    return product_int8(codes, scale, w, w_scale, status, gated, out_dtype or x.dtype)
+    # (the kernel ahead of the product is the tokens' own: the weights may be fetched before it is through)
+    return _product(codes, scale, w, w_scale, status, gated, out_dtype or x.dtype, 1)
 
 
 def lay_out_codes(w: torch.Tensor) -> torch.Tensor:
