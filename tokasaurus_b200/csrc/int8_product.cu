@@ -28,33 +28,111 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
   return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 
-constexpr int Q_THREADS = 256;
+// A block a row.  A thread's numbers (up to CHUNKS times eight, as they were loaded) stay in registers between the search for
+// the largest and the codes; what a row has beyond that is read again.  WIDE: rows start on 16-byte boundaries and are
+// read and written eight numbers at a time (their last few one by one).
+constexpr int CHUNKS = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(Q_THREADS)
+template <typename T, bool WIDE> struct Eight;
+template <> struct Eight<bf16, true> {
+  uint4 v;
+  __device__ void load(const bf16* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ float at(int i) const {
+    const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+    return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
+  }
+};
+template <> struct Eight<float, true> {
+  float4 a, b;
+  __device__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1]; }
+  __device__ float at(int i) const {
+    return i == 0 ? a.x : i == 1 ? a.y : i == 2 ? a.z : i == 3 ? a.w : i == 4 ? b.x : i == 5 ? b.y : i == 6 ? b.z : b.w;
+  }
+};
+template <typename T> struct Eight<T, false> {
+  T v[8];
+  __device__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = p[i];
+  }
+  __device__ float at(int i) const { return to_float(v[i]); }
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(1024)
 quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc, float* __restrict__ scale,
                      int K) {
-  __shared__ unsigned s_top[Q_THREADS / 32];
+  __shared__ unsigned s_top[32];
   // The product behind this kernel may fetch weights as soon as it has started: only then, when every kernel ahead of this
   // one (one that made those weights among them) is over.
   grid_dependency_wait();
   trigger_dependents();
   const T* row = x + (long long)blockIdx.x * ldx;
   int8_t* dst = codes + (long long)blockIdx.x * ldc;
+  const int eights = K >> 3, step = blockDim.x;
+  const int tail = (eights << 3) + threadIdx.x;  // the last K % 8 numbers: the first threads' own
+  Eight<T, WIDE> mine[CHUNKS];
   // magnitudes as integers: NaN > infinity > every number
   unsigned top = 0;
-  for (int k = threadIdx.x; k < K; k += Q_THREADS) top = max(top, __float_as_uint(to_float(row[k])) & 0x7fffffffu);
+  auto see = [&](float v) { top = max(top, __float_as_uint(v) & 0x7fffffffu); };
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c++) {
+    const int e = threadIdx.x + c * step;
+    if (e < eights) mine[c].load(row + 8 * e);
+  }
+  const float last = tail < K ? to_float(row[tail]) : 0.f;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c++)
+    if (threadIdx.x + c * step < eights) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) see(mine[c].at(i));
+    }
+  see(last);
+  for (int e = threadIdx.x + CHUNKS * step; e < eights; e += step) {
+    Eight<T, WIDE> v;
+    v.load(row + 8 * e);
+#pragma unroll
+    for (int i = 0; i < 8; i++) see(v.at(i));
+  }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < Q_THREADS / 32; i++) top = max(top, s_top[i]);
+  const int lane = threadIdx.x & 31;
+  top = __reduce_max_sync(0xffffffffu, lane < (step >> 5) ? s_top[lane] : 0u);
   const bool finite = top < 0x7f800000u;
   const float s = finite ? __uint_as_float(top) * ONE_127TH : NAN;
   const float inv = 1.f / s;
   const bool some = finite && s > 0.f;
-  for (int k = threadIdx.x; k < K; k += Q_THREADS) dst[k] = some ? (int8_t)code_of(to_float(row[k]), s, inv) : (int8_t)0;
+  auto put = [&](int e, const Eight<T, WIDE>& v) {
+    uint32_t w[2] = {0, 0};
+    if (some) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)(uint8_t)code_of(v.at(i), s, inv) << (8 * (i & 3));
+    }
+    *reinterpret_cast<uint2*>(dst + 8 * e) = make_uint2(w[0], w[1]);
+  };
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c++) {
+    const int e = threadIdx.x + c * step;
+    if (e < eights) put(e, mine[c]);
+  }
+  for (int e = threadIdx.x + CHUNKS * step; e < eights; e += step) {
+    Eight<T, WIDE> v;
+    v.load(row + 8 * e);
+    put(e, v);
+  }
+  if (tail < K) dst[tail] = some ? (int8_t)code_of(last, s, inv) : (int8_t)0;
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
+}
+
+template <typename T>
+int quantise(const void* x, long long ldx, void* codes, long long ldc, float* scale, int M, int K, cudaStream_t st) {
+  // two chunks of eight a thread at least; with four, 256 threads hold 8,192 numbers and 1,024 threads 32,768
+  int threads = ((K + 15) / 16 + 31) / 32 * 32;
+  threads = threads < 64 ? 64 : threads <= 256 ? threads : K <= 8192 ? 256 : 1024;
+  const bool wide = (((uintptr_t)x) & 15) == 0 && (M == 1 || ldx % (16 / (long long)sizeof(T)) == 0);
+  auto kernel = wide ? quantise_rows_kernel<T, true> : quantise_rows_kernel<T, false>;
+  return launch_pdl(kernel, dim3(M), dim3(threads), 0, st, (const T*)x, ldx, (int8_t*)codes, ldc, scale, K);
 }
 
 // ------------------------------------------------------------------------------------------------ shared by both products
@@ -495,6 +573,21 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
 #undef TKB_ARGS
 }
 
+// a, w: codes whose rows start on 16-byte boundaries (row strides lda, ldw in bytes).  weights_ready: the kernel ahead in the
+// stream is the one that makes the tokens' codes, so that no kernel that may still be running writes w.
+int product_any(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
+                long long ldo, int f32, int M, int N, int K, int gated, int weights_ready, int* status, cudaStream_t st) {
+  if (M <= 0 || N <= 0) return 0;
+  if (K <= 0 || K > 132103 || (gated && (N & 15)) || (lda & 15) || (ldw & 15) || (((uintptr_t)a) & 15) || (((uintptr_t)w) & 15)) return -2;
+  int rc = get_encode();
+  if (rc) return rc;
+  if (gated)
+    return f32 ? product<true, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
+               : product<true, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
+  return f32 ? product<false, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
+             : product<false, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
+}
+
 }  // namespace
 
 // codes [M, ldc] int8 and scale [M] of x [M, K] (float32: f32 != 0, else bfloat16; row stride ldx elements).
@@ -502,24 +595,22 @@ TKB_EXPORT int tkb_quantise_rows(const void* x, long long ldx, int f32, void* co
   if (M <= 0) return 0;
   if (K <= 0) return -2;
   cudaStream_t st = (cudaStream_t)st_;
-  if (f32)
-    return launch_pdl(quantise_rows_kernel<float>, dim3(M), dim3(Q_THREADS), 0, st, (const float*)x, ldx, (int8_t*)codes, ldc, (float*)scale, K);
-  return launch_pdl(quantise_rows_kernel<bf16>, dim3(M), dim3(Q_THREADS), 0, st, (const bf16*)x, ldx, (int8_t*)codes, ldc, (float*)scale, K);
+  return f32 ? quantise<float>(x, ldx, codes, ldc, (float*)scale, M, K, st) : quantise<bf16>(x, ldx, codes, ldc, (float*)scale, M, K, st);
+}
+
+// Both in one call: scratch has room for M float32 (padded to 16 bytes), then M rows of K codes padded to 16 bytes each.
+TKB_EXPORT int tkb_linear_int8(const void* x, long long ldx, int x_f32, const void* w, long long ldw, const float* w_scale, void* out,
+                               long long ldo, int f32, void* scratch, int M, int N, int K, int gated, int* status, void* st) {
+  if (M <= 0 || N <= 0) return 0;
+  float* scale = (float*)scratch;
+  char* codes = (char*)scratch + ((size_t)M * 4 + 15) / 16 * 16;
+  const long long ldc = ((long long)K + 15) / 16 * 16;
+  const int rc = tkb_quantise_rows(x, ldx, x_f32, codes, ldc, scale, M, K, st);
+  return rc ? rc : product_any(codes, ldc, scale, w, ldw, w_scale, out, ldo, f32, M, N, K, gated, 1, status, (cudaStream_t)st);
 }
 
 // out [M, N] (gated: [M, N / 2], rows of w interleaving gate and up in eights) float32 or bfloat16, row stride ldo elements.
-// a, w: codes whose rows start on 16-byte boundaries (row strides lda, ldw in bytes).  weights_ready: the kernel ahead in the
-// stream is tkb_quantise_rows (of the tokens), so that no kernel that may still be running writes w.
 TKB_EXPORT int tkb_int8_product(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale,
-                                void* out, long long ldo, int f32, int M, int N, int K, int gated, int weights_ready, int* status, void* st_) {
-  if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K > 132103 || (gated && (N & 15)) || (lda & 15) || (ldw & 15) || (((uintptr_t)a) & 15) || (((uintptr_t)w) & 15)) return -2;
-  int rc = get_encode();
-  if (rc) return rc;
-  cudaStream_t st = (cudaStream_t)st_;
-  if (gated)
-    return f32 ? product<true, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
-               : product<true, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
-  return f32 ? product<false, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
-             : product<false, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
+                                void* out, long long ldo, int f32, int M, int N, int K, int gated, int* status, void* st) {
+  return product_any(a, lda, a_scale, w, ldw, w_scale, out, ldo, f32, M, N, K, gated, 0, status, (cudaStream_t)st);
 }

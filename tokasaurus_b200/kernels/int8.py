@@ -15,10 +15,35 @@ from ctypes import c_float, c_int
 
 import torch
 
-from tokasaurus_b200.kernels.ops import _check, _fn, _libs, _need, _need_cuda, _ptr, _stream, _suffix, check_head_dim
+from tokasaurus_b200.kernels import ops
+from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, _need_cuda, _ptr, _stream, _suffix, check_head_dim
 
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
 c_longlong = ctypes.c_longlong
+
+
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_ARGS = {
+    "tkb_quantise_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _P),
+    "tkb_int8_product": (_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P),
+    "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _P, _P),
+    "tkb_attn_kv8_scratch": (_I,) * 6,
+    "tkb_linear_int8": (_P, _L, _I, _P, _L, _P, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P),
+}
+_functions: dict = {}
+
+
+def _entry(source: str, name: str, head_dim: int = 0):
+    """A launcher whose argument types are declared once: plain numbers go straight in (a step's small calls cost more on the
+    host than on the GPU otherwise).  ``head_dim``: of a source that is compiled by head size."""
+    f = _functions.get((name, head_dim))
+    if f is None:
+        f = _fn(_libs.get(source, **({"TKB_HD": head_dim} if head_dim else {})), name)
+        f.argtypes = _ARGS[name]
+        if name.endswith("_scratch"):
+            f.restype = _L
+        _functions[(name, head_dim)] = f
+    return f
 
 
 def _is_f32(dtype: torch.dtype) -> int:
@@ -38,18 +63,39 @@ def _code_rows(rows: int, k: int, device) -> torch.Tensor:
     return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
 
 
+def _check_rows(what: str, x: torch.Tensor) -> None:
+    if not (x.dim() == 2 and x.shape[1] >= 1 and (x.stride(1) == 1 or x.shape[1] == 1)):
+        raise KernelError(f"{what}: rows of numbers that lie together")
+
+
+def _check_codes(what: str, t: torch.Tensor, scale: torch.Tensor) -> None:
+    if not (t.dtype == torch.int8 and t.dim() == 2 and 1 <= t.shape[1] <= MAX_K):
+        raise KernelError(f"{what}: int8 rows of 1 to {MAX_K} codes (the sum of a longer row's products need not fit 32 bits)")
+    n, k = t.shape
+    if not ((t.stride(1) == 1 or k == 1) and (n <= 1 or t.stride(0) % 16 == 0) and t.data_ptr() % 16 == 0):
+        raise KernelError(f"{what}: rows of codes lie on 16-byte boundaries (quantise_rows and lay_out_codes leave them so)")
+    if not (scale.dtype == torch.float32 and scale.numel() == n and scale.is_contiguous()):
+        raise KernelError(f"{what}: a float32 scale a row of codes")
+
+
+def _check_product(what: str, k: int, w: torch.Tensor, gated: bool) -> None:
+    if w.shape[1] != k or w.shape[0] < 1:
+        raise KernelError(f"{what}: as many numbers in a row of tokens as of weights [N, K]")
+    if gated and w.shape[0] % 16:
+        raise KernelError(f"{what}: gated weights come in groups of 16 rows")
+
+
 def quantise_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes int8 [M, K] (rows on 16-byte boundaries) and scales float32 [M] of the rows of ``x`` (bfloat16 or float32):
     a step's tokens, or a weight matrix [out, in] that ``linear_int8`` then takes."""
     _need_cuda(x)
-    _need(x.dim() == 2 and x.shape[1] >= 1 and (x.stride(1) == 1 or x.shape[1] == 1), "quantise_rows: rows of numbers that lie together")
+    _check_rows("quantise_rows", x)
     f32 = _is_f32(x.dtype)
     M, K = x.shape
     codes = _code_rows(M, K, x.device)
     scale = torch.empty((M,), dtype=torch.float32, device=x.device)
-    _check(_fn(_libs.get("int8_product.cu"), "tkb_quantise_rows")(
-        _ptr(x), c_longlong(x.stride(0)), c_int(f32), _ptr(codes), c_longlong((K + 15) // 16 * 16), _ptr(scale), c_int(M), c_int(K),
-        _stream()), "quantise_rows")
+    _check(_entry("int8_product.cu", "tkb_quantise_rows")(
+        x.data_ptr(), x.stride(0), f32, codes.data_ptr(), (K + 15) // 16 * 16, scale.data_ptr(), M, K, _stream()), "quantise_rows")
     return codes, scale
 
 
@@ -58,37 +104,44 @@ def product_int8(codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_sc
     """``(codes @ w^T) * scale[:, None] * w_scale`` of 8-bit codes [M, K] and [N, K] (rows on 16-byte boundaries); the sums
     are exact.  ``gated``: ``w`` and ``w_scale`` interleave gate and up rows (``ops.interleave_gate_up``), the result is
     silu(gate) * up [M, N / 2]."""
-    return _product(codes, scale, w, w_scale, status, gated, out_dtype, 0)
-
-
-def _product(codes, scale, w, w_scale, status, gated, out_dtype, weights_ready: int) -> torch.Tensor:
+    what = "product_int8"
     _need_cuda(codes, scale, w, w_scale, status)
-    _need(codes.dtype == torch.int8 and w.dtype == torch.int8 and codes.dim() == 2 and w.dim() == 2 and codes.shape[1] == w.shape[1],
-          "product_int8: int8 codes [M, K] and [N, K]")
+    _check_codes(what, codes, scale)
+    _check_codes(what, w, w_scale)
     M, K = codes.shape
     N = w.shape[0]
-    _need(1 <= K <= MAX_K and N >= 1, f"product_int8: 1 to {MAX_K} numbers a row (their sum has to fit 32 bits)")
-    for t, what in ((codes, "tokens"), (w, "weights")):
-        _need((t.stride(1) == 1 or K == 1) and (t.shape[0] <= 1 or t.stride(0) % 16 == 0) and t.data_ptr() % 16 == 0,
-              f"product_int8: rows of the {what}' codes lie on 16-byte boundaries (quantise_rows and lay_out_codes leave them so)")
-    _need(scale.dtype == torch.float32 and scale.is_contiguous() and scale.numel() == M, "product_int8: token scales float32 [M]")
-    _need(w_scale.dtype == torch.float32 and w_scale.is_contiguous() and w_scale.numel() == N, "product_int8: channel scales float32 [N]")
-    _need(not gated or N % 16 == 0, "product_int8: gated weights come in groups of 16 rows")
-    out = torch.empty((M, N // 2 if gated else N), dtype=out_dtype, device=codes.device)
-    _check(_fn(_libs.get("int8_product.cu"), "tkb_int8_product")(
-        _ptr(codes), c_longlong(_code_stride(codes)), _ptr(scale), _ptr(w), c_longlong(_code_stride(w)), _ptr(w_scale), _ptr(out),
-        c_longlong(out.shape[1]), c_int(_is_f32(out_dtype)), c_int(M), c_int(N), c_int(K), c_int(1 if gated else 0), c_int(weights_ready),
-        _ptr(status), _stream()), "product_int8")
+    _check_product(what, K, w, gated)
+    cols = N // 2 if gated else N
+    out = torch.empty((M, cols), dtype=out_dtype, device=codes.device)
+    _check(_entry("int8_product.cu", "tkb_int8_product")(
+        codes.data_ptr(), _code_stride(codes), scale.data_ptr(), w.data_ptr(), _code_stride(w), w_scale.data_ptr(), out.data_ptr(), cols,
+        _is_f32(out_dtype), M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
     return out
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status: torch.Tensor, gated: bool = False,
                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ (w * w_scale[:, None])^T`` with ``x`` [M, K] (bfloat16 or float32) brought to 8 bits token by token and the
-    products summed in integers.  The result has ``out_dtype`` (``x``'s if None)."""
-    codes, scale = quantise_rows(x)
-    # (the kernel ahead of the product is the tokens' own: the weights may be fetched before it is through)
-    return _product(codes, scale, w, w_scale, status, gated, out_dtype or x.dtype, 1)
+    products summed in integers (``quantise_rows``, then ``product_int8``).  The result has ``out_dtype`` (``x``'s if None)."""
+    what = "linear_int8"
+    _need_cuda(x, w, w_scale, status)
+    _check_rows(what, x)
+    _check_codes(what, w, w_scale)
+    M, K = x.shape
+    N = w.shape[0]
+    _check_product(what, K, w, gated)
+    x_dtype = x.dtype
+    out_dtype = out_dtype or x_dtype
+    x_f32, f32 = _is_f32(x_dtype), _is_f32(out_dtype)
+    cols = N // 2 if gated else N
+    device = x.device
+    out = torch.empty((M, cols), dtype=out_dtype, device=device)
+    scratch = torch.empty(((M * 4 + 15) // 16 * 16 + M * ((K + 15) // 16 * 16),), dtype=torch.int8, device=device)
+    _check(_entry("int8_product.cu", "tkb_linear_int8")(
+        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), _code_stride(w), w_scale.data_ptr(), out.data_ptr(), cols, f32, scratch.data_ptr(),
+        M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
+    ops.LAUNCHES += 1  # two kernels
+    return out
 
 
 def lay_out_codes(w: torch.Tensor) -> torch.Tensor:
@@ -192,8 +245,15 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     _need(q_start.numel() >= n and kv_len.numel() >= n and page_indptr.numel() > n, f"{what}: a start, a length and pages for every request")
     _need(window is None or window >= 1, f"{what}: a window of one key at least")
     _need(max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n, f"{what}: bounds")
-    _check(_fn(_libs.get("attention_kv8.cu"), "tkb_attn_kv8")(
-        _ptr(q), c_longlong(_stride0(q)), _ptr(out), c_longlong(_stride0(out)), c_int(f32), _ptr(kcache), _ptr(vcache), _ptr(k_scale),
-        _ptr(v_scale), _ptr(q_start), _ptr(q_len), _ptr(kv_len), _ptr(page_indptr), _ptr(page_ids), c_int(n), c_int(max_q_len),
-        c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(page_size), c_float(scale), c_int(window or 0), c_int(kcache.shape[0]),
-        _ptr(status), _stream()), what)
+    T = q.shape[0]
+    if n == 0 or T == 0:
+        return
+    group = n_heads // n_kv_heads
+    singles = min(single_tokens, T)
+    scratch = torch.empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(n, singles, T, max_kv_len, n_kv_heads, group),),
+                          dtype=torch.uint8, device=q.device)
+    _check(_entry("attention_kv8.cu", "tkb_attn_kv8", head_dim)(
+        q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
+        scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0],
+        status.data_ptr(), _stream()), what)
