@@ -10,21 +10,24 @@
 //     S^T = K Q^T    mma.sync 16 keys x 8 columns x 32 in 8-bit integers: the cache's codes go in as they lie there, a query as
 //                    two pieces (three in float32 steps) of a 16-bit (24-bit) fixed-point number whose unit is its largest / 32,512
 //                    (/ 8,323,072).  The sums are exact; the rounding is 2^-16 of a query's largest number
-//     O^T += V^T W   mma.sync 16 numbers x 8 columns x 16 in halves, W = 2^(s + log2 sv - M): the values' scales are in the
+//     O^T += V^T W   mma.sync 16 numbers x 8 columns x 16 in halves, W = 2^(s - m) sv 2^(m - M): the values' scales are in the
 //                    weights, and a code is made a half exactly (its bits under an exponent of 2^10, less 1,152)
 // Keys on the rows: 16 of them fill an instruction whose 8 columns a group of heads fills, where queries as rows would leave
 // three quarters of the products empty.  Scores, sums and output are float32.  s and s + log2 sv have references of their own
-// (m and M; a column's largest so far, moved when topped by 2^8): weights are at most 2^8 in half precision whatever the
+// (m and M; a column's largest when last moved, which it is before a weight tops 2^8): weights fit half precision whatever the
 // scales are, and lose nothing that the largest of them would not drown.  In float32 steps weights go in as two halves (22 bits).
 //
 // Work is cut on the device: the tiles of all items (request, column tile) stand in a row, and each of the blocks of a kv head
 // takes an even share of them, whatever the requests' lengths are; what a share holds of an item that it does not hold whole
-// is left as (O, M, m, l) and put together by a second small kernel, in the order of the shares (same bits every time).
-// For short contexts shares are rounded to whole items and the second kernel is not launched.
+// is left as (O, M, m, l), and the block that leaves an item's last part puts the parts together, in the order of the shares
+// (same bits every time).  For short contexts shares are rounded to whole items and there are no parts.
 // Every wait is bounded (TKB_STATUS_WAIT_TIMEOUT).
 #include "tcgen05.cuh"
 #include "per_device.h"
 #include <cuda_fp16.h>
+
+#include <atomic>
+#include <chrono>
 
 #ifndef TKB_HD
 #error "compile with -DTKB_HD=<head size>"
@@ -36,27 +39,36 @@ namespace {
 
 constexpr int HD = TKB_HD;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size");
-constexpr int BKV = 64;              // keys a tile
-constexpr int WARPS = 4;             // 16 keys of a tile each
+constexpr int WARPS = 4;
 constexpr int THREADS = (WARPS + 1) * 32;
-constexpr int KV_BYTES = BKV * HD;
-constexpr int STAGES = HD <= 64 ? 4 : HD <= 128 ? 3 : 2;
 constexpr int DTILES = HD / 16;      // 16-row tiles of O^T; words of codes that a lane takes of a key
 constexpr int KSTEPS = (HD + 31) / 32;  // products along the head size
 constexpr bool SWIZZLES = HD == 64 || HD == 128;
+constexpr int WINDOW = 64;           // pages that are looked up together; a tile has no more
 constexpr float SLACK = 8.f;
+constexpr int WHOLE_KEYS = 512;       // up to so many keys a request's items are not cut
 constexpr float LOWEST = -1e30f;  // a reference before the first key
 
 __host__ __device__ constexpr int max_nt() { return HD <= 128 ? 2 : 1; }
 
+// GROUPS: groups of 16 keys that a warp takes of a tile at once.  Two where registers allow: the chains of one fill the gaps of
+// the other, and a tile's waits and references are shared (one group, tiles of 64: 64 requests of 2,100 keys 49 us).
 template <typename T, int NT> struct Layout {
+  static constexpr int GROUPS = NT == 1 && HD <= 128 ? 2 : 1;
+  static constexpr int BKV = 16 * GROUPS * WARPS;  // keys a tile
+  static constexpr int KV_BYTES = BKV * HD;
+  static constexpr int STAGES = HD <= 64 ? 8 / GROUPS : HD <= 128 ? 4 / GROUPS : 2;
+  static constexpr int BLOCKS = HD > 128 ? 1 : NT == 2 ? 2 : 3;  // blocks an SM
   static constexpr int QP = sizeof(T) == 4 ? 3 : 2;  // pieces of a query
   static constexpr int WP = sizeof(T) == 4 ? 2 : 1;  // pieces of a weight
   static constexpr int COLS = 8 * NT;
   static constexpr int RING = 2 * STAGES * KV_BYTES;
   static constexpr int QF = QP * KSTEPS * NT * 32 * 8;   // queries as the instructions take them
-  static constexpr int OUT = COLS * (HD + 4) * 4;            // output of the four warps together
-  static constexpr int BYTES = 1024 + RING + QF + OUT;
+  static constexpr int OUT = COLS * HD * 4;                  // output of the four warps together
+  static constexpr int PART = COLS * HD + 3 * COLS;          // floats of a part: output, M, m, l
+  static constexpr int KEYS = STAGES * BKV * 8;              // key's and value's scale of every page (key) in the ring
+  static constexpr int BYTES = 1024 + RING + QF + OUT + KEYS;
+  static_assert(BLOCKS * (BYTES + 2048) <= 228 * 1024 || BLOCKS == 1 || sizeof(T) == 4 || NT == 2, "shared memory of the blocks that an SM is meant to hold");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -75,6 +87,10 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8_new(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -96,25 +112,46 @@ __device__ __forceinline__ uint32_t rest_half(uint32_t h, float lo, float hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   return pack_half(lo - f.x, hi - f.y);
 }
-// The key (of a warp's 16) in row r of the products: rows 2c and 2c + 1 of a lane group stand in different halves of the
-// swizzle, so that neither the reads of K (rows next to one another) nor those of V (every second row) meet a bank twice.
-__device__ __forceinline__ int key_of_row(int r) { return (r & 8) | ((r & 1) ? (r & 6) ^ 5 : r & 6); }
+// The key (of a warp's 16) in row r of the products: an order in which neither the reads of K (neighbouring rows) nor those of V
+// (every second row) meet a bank twice under the swizzle.
+__device__ __forceinline__ int key_of_row(int r) { return HD == 64 ? r ^ ((r >> 1) & 1) : (r & 8) | ((r & 1) ? (r & 6) ^ 5 : r & 6); }
+// Where byte `at` of key k lies in the ring.  A 128-byte row is one key's of 128 codes or two keys' of 64; its 16-byte chunks are
+// exclusive-or the row's number, as TMA leaves them.
+__device__ __forceinline__ int place(int k, int at, bool swizzled) {
+  const int x = k * HD + at;
+  return SWIZZLES && swizzled ? x ^ ((HD == 128 ? k & 7 : (k >> 1) & 7) << 4) : x;
+}
 
 // O / l under their references.  Nothing seen: zeros.  Weights that were all zero (values' scales of zero) leave M where it was.
 __device__ __forceinline__ float last_factor(float M, float m, float l) {
   return l == 0.f ? 0.f : M == LOWEST ? 1.f : ex2(M - m) / l;
 }
 
+// Where results go, and how columns stand for tokens and heads.
+struct Out {
+  void* rows;
+  long long stride;
+  int group;
+  unsigned mul;  // 2^32 / group, rounded up
+  // n / group without a division's latency
+  __device__ __forceinline__ int token(int n) const {
+    if (group == 1) return n;
+    const int x = (int)__umulhi((unsigned)n, mul);
+    return x - (x * group > n);
+  }
+};
+
 struct Args {
   const void* q;
-  void* out;
+  Out out;
   const int8_t *kcache, *vcache;
   const float *k_scale, *v_scale;
   const int *q_start, *q_len, *kv_len, *page_indptr, *page_ids;
-  float* parts;          // [kv heads][blocks][2][Layout::COLS][HD + 4]: O, M, m, l
-  int* base;             // [requests]: where a request's tiles start in the row of all tiles; [requests]: how many there are
-  long long q_stride, out_stride;
-  int n_seqs, group, nkv, ps, ps_shift, window, num_pages, which, whole, tma_rows;
+  float* parts;          // [kv heads][blocks][2][Layout::PART]
+  unsigned long long* arrived;  // [kv heads][blocks]: parts left of the item that is cut at the end of a share, under this launch's tag
+  unsigned long long tag;
+  long long q_stride;
+  int n_seqs, nkv, ps, ps_shift, window, num_pages, which, whole, tma_rows;
   float scale_log2;
   int* status;
 };
@@ -122,13 +159,16 @@ constexpr int SINGLE = 1, PORTION = 2;  // `which`
 
 // One request's part of the work.
 struct Request {
-  int s, q_len, kv_len, col_tiles, k0, tiles;
-  __device__ __forceinline__ bool load(const Args& a, int s_, int cols) {
+  int s, q_len, kv_len, q_start, table, col_tiles, k0, tiles;
+  template <typename L> __device__ __forceinline__ bool load(const Args& a, int s_) {
+    constexpr int BKV = L::BKV, cols = L::COLS;
     s = s_;
     q_len = a.q_len[s];
     kv_len = a.kv_len[s];
+    q_start = a.q_start[s];
+    table = a.page_indptr[s];
     if (q_len <= 0 || !(a.which & (q_len == 1 ? SINGLE : PORTION))) return false;
-    col_tiles = (q_len * a.group + cols - 1) / cols;
+    col_tiles = (q_len * a.out.group + cols - 1) / cols;
     const int first = a.window > 0 ? max(0, kv_len - q_len - a.window + 1) : 0;
     k0 = first & ~(BKV - 1);
     tiles = max(1, (kv_len - k0 + BKV - 1) / BKV);
@@ -149,6 +189,11 @@ struct Shares {
   }
 };
 
+// An item that goes over several shares: where it starts in the row of all tiles, its first share, its parts, its place.
+struct CutItem {
+  int at, b0, n, q_start, col0, cols;
+};
+
 // A block's share as it is walked: item after item, tile after tile.
 struct Walk {
   Request r;
@@ -157,7 +202,7 @@ struct Walk {
   int at, end;           // in the row of all tiles
   bool live, opens;      // opens: the share starts with this item
   __device__ __forceinline__ void clip() { tile_end = end - at < r.tiles - tile ? tile + (end - at) : r.tiles; }
-  __device__ __forceinline__ void next_item(const Args& a, int cols) {
+  template <typename L> __device__ __forceinline__ void next_item(const Args& a) {
     at += tile_end - tile;
     opens = false;
     live = at < end;
@@ -166,29 +211,138 @@ struct Walk {
     if (++ct == r.col_tiles) {
       ct = 0;
       int s = r.s + 1;
-      while (s < a.n_seqs && !r.load(a, s, cols)) s++;
+      while (s < a.n_seqs && !r.template load<L>(a, s)) s++;
       if (s >= a.n_seqs) { live = false; return; }
     }
     clip();
   }
 };
 
+// HD / 8 numbers that lie together of one column of a result in s_out's order: run i = g * COLS + column.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_run(const Out out, const float* res, int q_start, int col0, int cols, int i, float factor, int kvh) {
+  constexpr int W = HD / 8;
+  const int col = col0 + i % COLS, g = i / COLS;
+  if (col >= cols) return;
+  const int token = out.token(col);
+  T* dst = reinterpret_cast<T*>(out.rows) + (q_start + token) * out.stride + (long long)(kvh * out.group + col - token * out.group) * HD + g * W;
+  float x[W];
+#pragma unroll
+  for (int r = 0; r < W; r++) x[r] = res[r * 8 * COLS + i] * factor;
+  constexpr int VEC = 16 / sizeof(T);
+  if (W % VEC == 0 && (((uintptr_t)dst) & 15) == 0) {
+#pragma unroll
+    for (int r = 0; r < W; r += VEC) {
+      uint4 u;
+      if constexpr (sizeof(T) == 4) u = make_uint4(__float_as_uint(x[r]), __float_as_uint(x[r + 1]), __float_as_uint(x[r + 2]), __float_as_uint(x[r + 3]));
+      else u = make_uint4(pack_bf16(x[r], x[r + 1]), pack_bf16(x[r + 2], x[r + 3]), pack_bf16(x[(r + 4) % W], x[(r + 5) % W]), pack_bf16(x[(r + 6) % W], x[(r + 7) % W]));
+      *reinterpret_cast<uint4*>(dst + r) = u;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < W; r++) dst[r] = from_float<T>(x[r]);
+  }
+}
+
+// Parts of an item that have been left are counted in a word that starts as anything: a count counts under its launch's tag only
+// (tags are 54 bits, a new one for every launch; a graph's replays find the word emptied by the one before).  Every block that
+// will leave a part sees to the tag first, long before; then all add.
+__device__ __forceinline__ void put_tag(unsigned long long* word, unsigned long long tag) {
+  unsigned long long seen = *reinterpret_cast<volatile unsigned long long*>(word);
+  while ((seen >> 10) != tag) {
+    const unsigned long long was = atomicCAS(word, seen, tag << 10);
+    if (was == seen) break;
+    seen = was;
+  }
+}
+// One more part; whether it is the last of `n`.
+__device__ __forceinline__ bool arrive(unsigned long long* word, int n) {
+  const bool last = (int)(atomicAdd(word, 1ull) & 1023) == n - 1;
+  if (last) *reinterpret_cast<volatile unsigned long long*>(word) = 0;
+  return last;
+}
+
+// An item's `n` parts (the first stands at `first`, part i of the others at rest + 2 i parts) into its result, by 128 threads: the
+// columns' references and sums by every warp, then 32 parts at a time their factors through shared memory and four numbers of
+// each part a thread and load.  All in the order of the parts.
+constexpr int CHUNK = 32;
 template <typename T, int NT>
-__global__ void __launch_bounds__(THREADS, HD <= 64 ? 4 : HD <= 128 ? 3 : 1)
+__device__ __forceinline__ void join_parts(const Out out, const float* first, const float* rest, int n, float* s_out,
+                                           float (*s_fac)[8 * NT], int q_start, int col0, int cols, int kvh) {
+  using L = Layout<T, NT>;
+  constexpr int COLS = L::COLS, FOURS = (COLS * HD / 4 + 127) / 128;
+  constexpr bool EVEN = COLS * HD / 4 % 128 == 0;
+  const int lane = threadIdx.x & 31;
+  auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * L::PART; };
+  // a lane its column (lane % COLS), every (32 / COLS)-th part
+  float top = LOWEST, topM = LOWEST, sum = 0.f;
+#pragma unroll 4
+  for (int i = lane / COLS; i < n; i += 32 / COLS) {
+    const float* p = part(i) + COLS * HD + lane % COLS;
+    const float M = __ldcg(p), m = __ldcg(p + COLS), l = __ldcg(p + 2 * COLS), m2 = fmaxf(top, m);
+    topM = fmaxf(topM, M);
+    sum = sum * ex2(top - m2) + l * ex2(m - m2);
+    top = m2;
+  }
+  const float mine = top;
+#pragma unroll
+  for (int d = COLS; d < 32; d <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    topM = fmaxf(topM, __shfl_xor_sync(0xffffffffu, topM, d));
+  }
+  sum *= ex2(mine - top);
+#pragma unroll
+  for (int d = COLS; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float4 acc[FOURS];
+#pragma unroll
+  for (int f = 0; f < FOURS; f++) acc[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += CHUNK) {
+    const int k = min(CHUNK, n - i0);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int i = threadIdx.x / COLS; i < k; i += 128 / COLS) s_fac[i][lane % COLS] = ex2(__ldcg(part(i0 + i) + COLS * HD + lane % COLS) - topM);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 8
+    for (int i = 0; i < k; i++) {
+      const float4* p = reinterpret_cast<const float4*>(part(i0 + i));
+#pragma unroll
+      for (int f = 0; f < FOURS; f++) {
+        const int at = threadIdx.x + 128 * f;
+        if (EVEN || at < COLS * HD / 4) {
+          const float4 x = __ldcg(p + at), y = *reinterpret_cast<const float4*>(&s_fac[i][at * 4 % COLS]);
+          acc[f].x = fmaf(x.x, y.x, acc[f].x), acc[f].y = fmaf(x.y, y.y, acc[f].y);
+          acc[f].z = fmaf(x.z, y.z, acc[f].z), acc[f].w = fmaf(x.w, y.w, acc[f].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < FOURS; f++)
+    if (EVEN || threadIdx.x + 128 * f < COLS * HD / 4) reinterpret_cast<float4*>(s_out)[threadIdx.x + 128 * f] = acc[f];
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  const float factor = last_factor(topM, top, sum);  // (a thread's runs are all of column lane % COLS)
+  for (int i = threadIdx.x; i < COLS * 8; i += 128) store_run<T, COLS>(out, s_out, q_start, col0, cols, i, factor, kvh);
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(THREADS, (Layout<T, NT>::BLOCKS))
 attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
   using L = Layout<T, NT>;
-  constexpr int COLS = L::COLS, QP = L::QP, WP = L::WP;
+  constexpr int COLS = L::COLS, QP = L::QP, WP = L::WP, GROUPS = L::GROUPS, BKV = L::BKV, KV_BYTES = L::KV_BYTES, STAGES = L::STAGES;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
-  __shared__ float s_sk[STAGES][BKV], s_lsv[STAGES][BKV];
-  __shared__ int s_pos[STAGES][BKV];
   __shared__ float s_qs[COLS], s_M[WARPS][COLS], s_m[WARPS][COLS], s_l[WARPS][COLS];
   __shared__ int s_scan[THREADS / 32], s_offset, s_seq;
-  __shared__ bool s_whole[STAGES];  // every key of the tile is there
+  __shared__ Request s_first;
+  __shared__ CutItem s_cut[2];  // the item that the share starts with, and one that it ends with, if they are cut (n: their parts)
+  __shared__ uint32_t s_there[STAGES][BKV / 32];  // pages (keys) of a tile that the request still holds, a bit each
+  __shared__ bool s_whole[STAGES];                // all of them
+  __shared__ float s_most[STAGES];                // log2 of the tile's largest value scale
   __shared__ int failed;
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint32_t* qf = reinterpret_cast<uint32_t*>(ring + L::RING);
   float* s_out = reinterpret_cast<float*>(ring + L::RING + L::QF);
+  float (*s_sk)[BKV] = reinterpret_cast<float(*)[BKV]>(ring + L::RING + L::QF + L::OUT);
+  float (*s_sv)[BKV] = s_sk + STAGES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y;
   trigger_dependents();
@@ -199,6 +353,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     failed = 0;
     s_seq = -1;
+    s_cut[0].n = s_cut[1].n = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   grid_dependency_wait();
@@ -209,7 +364,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   int mine = 0;
   Request rq;
   for (int s = lo; s < hi; s++)
-    if (rq.load(a, s, COLS)) mine += rq.work();
+    if (rq.load<L>(a, s)) mine += rq.work();
   int before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -230,30 +385,22 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   if (start >= before && start < before + mine) {
     int at = before;
     for (int s = lo; s < hi; s++)
-      if (rq.load(a, s, COLS)) {
+      if (rq.load<L>(a, s)) {
         if (start < at + rq.work()) {
           s_seq = s;
           s_offset = start - at;
+          s_first = rq;
           break;
         }
         at += rq.work();
       }
   }
-  if (!a.whole && blockIdx.x == 0 && blockIdx.y == 0) {
-    // for the second kernel
-    int at = before;
-    for (int s = lo; s < hi; s++) {
-      a.base[s] = at;
-      if (rq.load(a, s, COLS)) at += rq.work();
-    }
-    if (threadIdx.x == 0) a.base[a.n_seqs] = total;
-  }
   __syncthreads();
   Walk w;
   w.live = s_seq >= 0 && start < end;
   if (w.live) {
-    w.r.load(a, s_seq, COLS);
-    w.ct = s_offset / w.r.tiles;
+    w.r = s_first;
+    w.ct = w.r.col_tiles == 1 ? 0 : s_offset / w.r.tiles;
     w.tile = s_offset - w.ct * w.r.tiles;
     w.at = start;
     w.end = end;
@@ -261,7 +408,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     w.clip();
     if (a.whole) {
       // a share holds the items that start in it, whole
-      if (w.tile > 0) w.next_item(a, COLS);
+      if (w.tile > 0) w.next_item<L>(a);
       if (w.live) {
         w.end = 0x7fffffff;
         w.clip();
@@ -269,11 +416,11 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
   }
   // (whole items: the share is over with the first item that starts behind `end`)
-  auto more = [&]() { return w.live && (!a.whole || w.at < end); };
+  auto more = [&](const Walk& x) { return x.live && (!a.whole || x.at < end); };
 
   // keys that some column of the item sees, as tiles of the item
   auto visible = [&](int& t_lo, int& t_hi) {
-    const int tok_lo = w.ct * COLS / a.group, tok_hi = min(w.r.q_len - 1, (w.ct * COLS + COLS - 1) / a.group);
+    const int tok_lo = a.out.token(w.ct * COLS), tok_hi = min(w.r.q_len - 1, a.out.token(w.ct * COLS + COLS - 1));
     const int p0 = w.r.kv_len - w.r.q_len;
     const int first = a.window > 0 ? max(0, p0 + tok_lo - a.window + 1) : 0;
     t_lo = max(w.tile, (first - w.r.k0) / BKV);
@@ -286,77 +433,100 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     // a tile waits for no lookup.
     uint32_t it = 0;
     bool ok = true, bad = false;
-    for (; more() && ok; w.next_item(a, COLS)) {
+    for (; more(w) && ok; w.next_item<L>(a)) {
       int t_lo, t_hi;
       visible(t_lo, t_hi);
-      const int* table = a.page_ids + a.page_indptr[w.r.s];
-      const int last_page = (w.r.kv_len - 1) / a.ps;
+      const int* table = a.page_ids + w.r.table;
+      const int last_page = a.ps_shift >= 0 ? (w.r.kv_len - 1) >> a.ps_shift : (w.r.kv_len - 1) / a.ps;
       auto page_at = [&](int p) { return p <= last_page ? __ldg(table + p) : -1; };
       int base = -1, id[2], next_id[2] = {-1, -1};
-      float sk[2], lsv[2];
+      float sk[2], sv[2];
       for (int t = t_lo; t < t_hi; t++, it++) {
         const int st = it % STAGES;
         const int key0 = w.r.k0 + t * BKV, key1 = min(key0 + BKV, w.r.kv_len);
         const int page0 = a.ps_shift >= 0 ? key0 >> a.ps_shift : key0 / a.ps;
         const int page1 = a.ps_shift >= 0 ? (key1 - 1) >> a.ps_shift : (key1 - 1) / a.ps;
-        const bool fresh = base < 0 || page1 >= base + 64;
+        const bool fresh = base < 0 || page1 >= base + WINDOW;
         if (fresh) {
-          const bool follows = base >= 0 && page0 == base + 64;
+          const bool follows = base >= 0 && page0 == base + WINDOW;
           base = page0;
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             id[i] = checked_page(follows ? next_id[i] : page_at(base + lane + 32 * i), a.num_pages, bad);
             const long long block = (long long)max(id[i], 0) * a.nkv + kvh;
             sk[i] = a.k_scale[block];
-            lsv[i] = a.v_scale[block];
-            next_id[i] = page_at(base + 64 + lane + 32 * i);
+            sv[i] = a.v_scale[block];
+            next_id[i] = page_at(base + WINDOW + lane + 32 * i);
           }
         }
         if (it >= STAGES && !mbar_wait(&empty[st], ((it / STAGES) - 1) & 1)) { ok = false; break; }
         unsigned char* dk = ring + st * 2 * KV_BYTES;
         uint32_t bytes = 0;
+        bool there = true;
+        float most_sv = 0.f;  // (a scale that is NaN makes its weights NaN wherever the reference stands)
+        // Scales and presence stand by page of the tile where a page is a power of two (entry of key k: k >> ps_shift), else by key.
+        const int pages = a.ps_shift >= 0 ? max(BKV >> a.ps_shift, 1) : page1 - page0 + 1;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const int p = page0 + lane + 32 * i, at = min(p - base, 63);
+          if (32 * i >= pages) break;
+          const int n = lane + 32 * i, p = page0 + n, at = min(p - base, WINDOW - 1);
           const int id0 = __shfl_sync(0xffffffffu, id[0], at & 31), id1 = __shfl_sync(0xffffffffu, id[1], at & 31);
           const int page = at < 32 ? id0 : id1;
-          if (p <= page1 && page >= 0) {
+          const bool real = p <= page1 && page >= 0;
+          if (real) {
             const int from = max(key0, p * a.ps);
             const long long row = ((long long)page * a.nkv + kvh) * a.ps + (from - p * a.ps);
             unsigned char* dst = dk + (from - key0) * HD;
             if (a.tma_rows > 0) {
-              tma_load_2d(dst, &map_k, &full[st], 0, (int)row);
-              tma_load_2d(dst + KV_BYTES, &map_v, &full[st], 0, (int)row);
-              bytes += 2 * HD * a.tma_rows;
+              tma_load_2d(dst, &map_k, &full[st], 0, (int)(row * HD / 128));
+              tma_load_2d(dst + KV_BYTES, &map_v, &full[st], 0, (int)(row * HD / 128));
+              bytes += 2 * 128 * a.tma_rows;
             } else {
-              const uint32_t n = (min(key1, (p + 1) * a.ps) - from) * HD;
-              bulk_copy(dst, a.kcache + row * HD, n, &full[st]);
-              bulk_copy(dst + KV_BYTES, a.vcache + row * HD, n, &full[st]);
-              bytes += 2 * n;
+              const uint32_t size = (min(key1, (p + 1) * a.ps) - from) * HD;
+              bulk_copy(dst, a.kcache + row * HD, size, &full[st]);
+              bulk_copy(dst + KV_BYTES, a.vcache + row * HD, size, &full[st]);
+              bytes += 2 * size;
             }
           }
+          if (a.ps_shift >= 0) {
+            // (the codes are on their way; the scales of a window's first tile may still be)
+            const float sk0 = __shfl_sync(0xffffffffu, sk[0], at & 31), sk1 = __shfl_sync(0xffffffffu, sk[1], at & 31);
+            const float lv0 = __shfl_sync(0xffffffffu, sv[0], at & 31), lv1 = __shfl_sync(0xffffffffu, sv[1], at & 31);
+            const uint32_t mask = __ballot_sync(0xffffffffu, real);
+            if (n < pages) {
+              const float v = real ? (at < 32 ? lv0 : lv1) : 0.f;
+              s_sk[st][n] = real ? (at < 32 ? sk0 : sk1) : 0.f;
+              s_sv[st][n] = v;
+              most_sv = fmaxf(most_sv, v);
+              there &= real;
+            }
+            if (lane == 0) s_there[st][i] = mask;
+          }
         }
-        // (the codes are on their way; the scales of a window's first tile may still be)
-        if (fresh) lsv[0] = log2f(lsv[0]), lsv[1] = log2f(lsv[1]);
-        bool there = true;
+        if (a.ps_shift < 0) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          const int key = key0 + lane + 32 * i;
-          const int at = min((a.ps_shift >= 0 ? key >> a.ps_shift : key / a.ps) - base, 63);
-          const int id0 = __shfl_sync(0xffffffffu, id[0], at & 31), id1 = __shfl_sync(0xffffffffu, id[1], at & 31);
-          const float sk0 = __shfl_sync(0xffffffffu, sk[0], at & 31), sk1 = __shfl_sync(0xffffffffu, sk[1], at & 31);
-          const float lv0 = __shfl_sync(0xffffffffu, lsv[0], at & 31), lv1 = __shfl_sync(0xffffffffu, lsv[1], at & 31);
-          const bool real = (at < 32 ? id0 : id1) >= 0 && key < key1;
-          s_sk[st][lane + 32 * i] = at < 32 ? sk0 : sk1;
-          s_lsv[st][lane + 32 * i] = at < 32 ? lv0 : lv1;
-          s_pos[st][lane + 32 * i] = real ? key : 0x7fffffff;
-          there &= real;
+          for (int i = 0; i < BKV / 32; i++) {
+            const int key = key0 + lane + 32 * i, at = min(key / a.ps - base, WINDOW - 1);
+            const int id0 = __shfl_sync(0xffffffffu, id[0], at & 31), id1 = __shfl_sync(0xffffffffu, id[1], at & 31);
+            const float sk0 = __shfl_sync(0xffffffffu, sk[0], at & 31), sk1 = __shfl_sync(0xffffffffu, sk[1], at & 31);
+            const float lv0 = __shfl_sync(0xffffffffu, sv[0], at & 31), lv1 = __shfl_sync(0xffffffffu, sv[1], at & 31);
+            const bool real = (at < 32 ? id0 : id1) >= 0 && key < key1;
+            const float v = real ? (at < 32 ? lv0 : lv1) : 0.f;
+            s_sk[st][lane + 32 * i] = real ? (at < 32 ? sk0 : sk1) : 0.f;
+            s_sv[st][lane + 32 * i] = v;
+            most_sv = fmaxf(most_sv, v);
+            const uint32_t mask = __ballot_sync(0xffffffffu, real);
+            if (lane == 0) s_there[st][i] = mask;
+            there &= real;
+          }
         }
         there = __all_sync(0xffffffffu, there);
         bytes = __reduce_add_sync(0xffffffffu, bytes);
+        most_sv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_sv)));  // (none is negative)
         __syncwarp();
         if (lane == 0) {
           s_whole[st] = there;
+          s_most[st] = __log2f(most_sv);
           if (bytes) mbar_expect_tx(&full[st], bytes);
           else mbar_arrive(&full[st]);
         }
@@ -367,37 +537,50 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   } else {
     // ---------------- scores, weights, output
     const int g = lane >> 2, c = lane & 3;
-    const int row0 = warp * 16 + key_of_row(g);  // this lane's key rows of a tile: row0, row0 + 8
-    uint32_t it = 0;
-    bool ok = true;
-    for (; more(); w.next_item(a, COLS)) {
-      const int cols = w.r.q_len * a.group, col0 = w.ct * COLS, p0 = w.r.kv_len - w.r.q_len;
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the item before is through with the queries and s_out
-      for (int j = warp; j < COLS; j += WARPS) {
-        const int col = col0 + j;
-        const bool real = col < cols;
-        const T* src = reinterpret_cast<const T*>(a.q) + (a.q_start[w.r.s] + (real ? col / a.group : 0)) * a.q_stride +
-                       (long long)(kvh * a.group + (real ? col % a.group : 0)) * HD;
-        constexpr int N4 = (HD / 4 + 31) / 32;  // four numbers (a word of codes) a lane and turn
-        float v[N4][4];
-        unsigned top = 0;
+    const int key_row = key_of_row(g);  // this lane's key rows of a group: key_row, key_row + 8
+    constexpr int MINE = COLS / WARPS;  // columns whose queries (and results) a warp brings in (out)
+    constexpr int N4 = (HD / 4 + 31) / 32;  // four numbers (a word of codes) of a query a lane and turn
+    float raw[MINE][N4][4];
+    auto load_queries = [&](const Walk& x) {
+#pragma unroll
+      for (int y = 0; y < MINE; y++) {
+        const int col = x.ct * COLS + warp + WARPS * y;
+        const bool real = col < x.r.q_len * a.out.group;
+        const int token = real ? a.out.token(col) : 0, head = real ? col - token * a.out.group : 0;
+        const T* src = reinterpret_cast<const T*>(a.q) + (x.r.q_start + token) * a.q_stride + (long long)(kvh * a.out.group + head) * HD;
 #pragma unroll
         for (int i = 0; i < N4; i++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int d = (lane + 32 * i) * 4 + e;
-            v[i][e] = real && d < HD ? to_float(src[d]) : 0.f;
-            top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+            raw[y][i][e] = real && d < HD ? to_float(src[d]) : 0.f;
           }
+      }
+    };
+    if (more(w)) load_queries(w);
+    auto holds_whole = [](const Walk& x) { return x.tile == 0 && x.tile_end == x.r.tiles; };
+    uint32_t it = 0;
+    bool ok = true;
+    while (more(w)) {
+      const int cols = w.r.q_len * a.out.group, col0 = w.ct * COLS, p0 = w.r.kv_len - w.r.q_len;
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the item before is through with the queries and s_out
+#pragma unroll
+      for (int y = 0; y < MINE; y++) {
+        const int j = warp + WARPS * y;
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < N4; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(raw[y][i][e]) & 0x7fffffffu);
         top = __reduce_max_sync(0xffffffffu, top);
         // by a power of two to [1, 2) (what is below 2^-126 stays there), then to the fixed point's unit
         const int e = max(1, (int)(top >> 23)) - 127;
-        const float down = __uint_as_float(e == 127 ? 0x00400000u : (unsigned)(127 - e) << 23), up = __uint_as_float(e == -126 ? 0x00800000u : (unsigned)(127 + e) << 23);
+        const float down = __uint_as_float(e == 127 ? 0x00400000u : (unsigned)(127 - e) << 23), up = __uint_as_float((unsigned)(127 + e) << 23);
         const float most = __uint_as_float(top) * down;
         const float units = QP == 3 ? 8323072.f : 32512.f;
         const bool some = top > 0 && top < 0x7f800000u;
-        const float f = some ? units / most : 0.f;
-        if (lane == 0) s_qs[j] = top < 0x7f800000u ? a.scale_log2 * (most / units) * up : NAN;
+        const float f = some ? __fdividef(units, most) : 0.f;
+        if (lane == 0) s_qs[j] = top < 0x7f800000u ? a.scale_log2 * (most * (1.f / units)) * up : NAN;
 #pragma unroll
         for (int i = 0; i < N4; i++) {
           const int word = lane + 32 * i;
@@ -405,7 +588,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             uint32_t piece[QP] = {};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-              int x = some ? __float2int_rn(v[i][b] * down * f) : 0;
+              int x = some ? __float2int_rn(raw[y][i][b] * down * f) : 0;
 #pragma unroll
               for (int p = QP - 1; p >= 0; p--) {
                 const int low = p == 0 ? x : (int)(int8_t)(x & 0xff);
@@ -421,7 +604,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      float qs[NT][2], m[NT][2], M[NT][2], l[NT][2], o[DTILES][NT][4];
+      float qs[NT][2], m[NT][2], M[NT][2], to_M[NT][2], l[NT][2], o[DTILES][NT][4];  // to_M: 2^(m - M)
       int pos[NT][2];  // the last key that a column sees (columns behind the last: as it)
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -429,9 +612,9 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         for (int e = 0; e < 2; e++) {
           const int j = n * 8 + 2 * c + e;
           qs[n][e] = s_qs[j];
-          pos[n][e] = p0 + min(col0 + j, cols - 1) / a.group;
+          pos[n][e] = p0 + a.out.token(min(col0 + j, cols - 1));
           m[n][e] = M[n][e] = LOWEST;
-          l[n][e] = 0.f;
+          l[n][e] = to_M[n][e] = 0.f;
         }
 #pragma unroll
       for (int k = 0; k < DTILES; k++)
@@ -439,178 +622,212 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int e = 0; e < 4; e++) o[k][n][e] = 0.f;
-
       uint2 q_own[NT == 1 ? QP * KSTEPS : 1];  // one column tile's queries stay in registers
       if (NT == 1) {
 #pragma unroll
         for (int i = 0; i < (NT == 1 ? QP * KSTEPS : 1); i++) q_own[i] = reinterpret_cast<const uint2*>(qf)[i * 32 + lane];
       }
+      if (threadIdx.x == 0 && !holds_whole(w)) {
+        const int at = w.at - w.tile, b0 = shares.of(at);
+        s_cut[w.opens ? 0 : 1] = {at, b0, shares.of(at + w.r.tiles - 1) - b0 + 1, w.r.q_start, col0, cols};
+        put_tag(a.arrived + (long long)kvh * gridDim.x + b0, a.tag);
+      }
       int t_lo, t_hi;
       visible(t_lo, t_hi);
       // tiles that every column sees whole, if their pages are there
-      const int whole_lo = a.window > 0 ? p0 + min(w.r.q_len - 1, (col0 + COLS - 1) / a.group) - a.window + 1 : 0;
-      const int whole_hi = p0 + col0 / a.group - BKV + 1;
+      const int whole_lo = a.window > 0 ? p0 + min(w.r.q_len - 1, a.out.token(col0 + COLS - 1)) - a.window + 1 : 0;
+      const int whole_hi = p0 + a.out.token(col0) - BKV + 1;
+      const int last_pos = p0 + a.out.token(min(col0 + COLS - 1, cols - 1));
       for (int t = t_lo; t < t_hi; t++, it++) {
         const int st = it % STAGES, key0 = w.r.k0 + t * BKV;
         ok = ok && mbar_wait(&full[st], (it / STAGES) & 1);
         if (!ok) break;
-        const unsigned char* kt = ring + st * 2 * KV_BYTES;
-        const unsigned char* vt = kt + KV_BYTES;
-        [[maybe_unused]] const bool swz = SWIZZLES && a.tma_rows > 0;
-        // S^T
-        uint32_t k0[DTILES + 1], k1[DTILES + 1];
-        if constexpr (HD % 64 == 0) {
-          // the swizzle of rows of 128 (64) bytes: 16-byte chunks exclusive-or the row (half the row)
-          const int x = !swz ? 0 : HD == 128 ? row0 & 7 : (row0 >> 1) & 3;
+        if (key0 + warp * 16 * GROUPS <= last_pos) {  // (else none of this warp's keys is seen)
+          const unsigned char* kt = ring + st * 2 * KV_BYTES + warp * 16 * GROUPS * HD;
+          const unsigned char* vt = kt + KV_BYTES;
+          [[maybe_unused]] const bool swz = SWIZZLES && a.tma_rows > 0;
+          float s[GROUPS][NT][4], sv[GROUPS][2], top = -INFINITY;
+          // S^T
 #pragma unroll
-          for (int i = 0; i < HD / 64; i++) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kt + row0 * HD + (((4 * i + c) ^ x) << 4));
-            const uint4 v = *reinterpret_cast<const uint4*>(kt + (row0 + 8) * HD + (((4 * i + c) ^ x) << 4));
-            k0[4 * i] = u.x, k0[4 * i + 1] = u.y, k0[4 * i + 2] = u.z, k0[4 * i + 3] = u.w;
-            k1[4 * i] = v.x, k1[4 * i + 1] = v.y, k1[4 * i + 2] = v.z, k1[4 * i + 3] = v.w;
-          }
-        } else {
+          for (int G = 0; G < GROUPS; G++) {
+            const unsigned char* row = kt + G * 16 * HD;
+            uint32_t k0[DTILES + 1], k1[DTILES + 1];
+            if constexpr (HD % 64 == 0) {
 #pragma unroll
-          for (int i = 0; i < DTILES; i++) {
-            k0[i] = *reinterpret_cast<const uint32_t*>(kt + row0 * HD + i * 16 + c * 4);
-            k1[i] = *reinterpret_cast<const uint32_t*>(kt + (row0 + 8) * HD + i * 16 + c * 4);
-          }
-        }
-        k0[DTILES] = k1[DTILES] = 0;  // (an odd number of words: the last product's second half)
-        float s[NT][4];
+              for (int i = 0; i < HD / 64; i++) {
+                const uint4 u = *reinterpret_cast<const uint4*>(row + place(key_row, 64 * i + 16 * c, swz));
+                const uint4 v = *reinterpret_cast<const uint4*>(row + place(key_row + 8, 64 * i + 16 * c, swz));
+                k0[4 * i] = u.x, k0[4 * i + 1] = u.y, k0[4 * i + 2] = u.z, k0[4 * i + 3] = u.w;
+                k1[4 * i] = v.x, k1[4 * i + 1] = v.y, k1[4 * i + 2] = v.z, k1[4 * i + 3] = v.w;
+              }
+            } else {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          int sum[QP][4] = {};
-#pragma unroll
-          for (int p = 0; p < QP; p++)
-#pragma unroll
-            for (int i = 0; i < KSTEPS; i++) {
-              const uint2 b = NT == 1 ? q_own[NT == 1 ? p * KSTEPS + i : 0] : reinterpret_cast<const uint2*>(qf)[((p * KSTEPS + i) * NT + n) * 32 + lane];
-              mma8(sum[p], k0[2 * i], k1[2 * i], k0[2 * i + 1], k1[2 * i + 1], b.x, b.y);
+              for (int i = 0; i < DTILES; i++) {
+                k0[i] = *reinterpret_cast<const uint32_t*>(row + key_row * HD + i * 16 + c * 4);
+                k1[i] = *reinterpret_cast<const uint32_t*>(row + (key_row + 8) * HD + i * 16 + c * 4);
+              }
             }
+            k0[DTILES] = k1[DTILES] = 0;  // (an odd number of words: the last product's second half)
+            const int kr = warp * 16 * GROUPS + G * 16 + key_row;
+            const int i0 = kr >> max(a.ps_shift, 0), i1 = (kr + 8) >> max(a.ps_shift, 0);
+            const float sk0 = s_sk[st][i0], sk1 = s_sk[st][i1];
+            sv[G][0] = s_sv[st][i0], sv[G][1] = s_sv[st][i1];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float low = (float)(sum[QP - 2][e] * 256 + sum[QP - 1][e]);
-            s[n][e] = QP == 3 ? fmaf((float)sum[0][e], 65536.f, low) : low;
-          }
-        }
-        // scores in powers of two less their reference, and the weights' exponents less theirs; what a column does not see has none
-        const float sk0 = s_sk[st][row0], sk1 = s_sk[st][row0 + 8], lv0 = s_lsv[st][row0], lv1 = s_lsv[st][row0 + 8];
-        float z[NT][4], top = -INFINITY;
+            for (int n = 0; n < NT; n++) {
+              int sum[QP][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+              for (int p = 0; p < QP; p++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            s[n][e] *= (e < 2 ? sk0 : sk1) * qs[n][e & 1];
-            z[n][e] = s[n][e] + (e < 2 ? lv0 : lv1);
-          }
-        if (!(s_whole[st] && key0 >= whole_lo && key0 <= whole_hi)) {
-          const int kp0 = s_pos[st][row0], kp1 = s_pos[st][row0 + 8];
+                for (int i = 0; i < KSTEPS; i++) {
+                  const uint2 b = NT == 1 ? q_own[NT == 1 ? p * KSTEPS + i : 0] : reinterpret_cast<const uint2*>(qf)[((p * KSTEPS + i) * NT + n) * 32 + lane];
+                  if (i == 0) mma8_new(sum[p], k0[0], k1[0], k0[1], k1[1], b.x, b.y);
+                  else mma8(sum[p], k0[2 * i], k1[2 * i], k0[2 * i + 1], k1[2 * i + 1], b.x, b.y);
+                }
+              // scores in powers of two
 #pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const int kp = e < 2 ? kp0 : kp1, q = pos[n][e & 1];
-              if (kp > q || (a.window > 0 && kp <= q - a.window)) s[n][e] = z[n][e] = -INFINITY;
+              for (int e = 0; e < 4; e++) {
+                const float low = (float)(sum[QP - 2][e] * 256 + sum[QP - 1][e]);
+                s[G][n][e] = (QP == 3 ? fmaf((float)sum[0][e], 65536.f, low) : low) * ((e < 2 ? sk0 : sk1) * qs[n][e & 1]);
+              }
             }
-        }
+          }
+          const bool masked = !(s_whole[st] && key0 >= whole_lo && key0 <= whole_hi);
+          if (masked) {  // what a column does not see has no score
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int G = 0; G < GROUPS; G++) {
+              const int kr = warp * 16 * GROUPS + G * 16 + key_row;
+              const int i0 = kr >> max(a.ps_shift, 0), i1 = (kr + 8) >> max(a.ps_shift, 0);
+              // (a key on a page that is gone stands behind every column)
+              const int kp0 = (s_there[st][i0 >> 5] >> (i0 & 31)) & 1 ? key0 + kr : 0x7fffffff;
+              const int kp1 = (s_there[st][i1 >> 5] >> (i1 & 31)) & 1 ? key0 + kr + 8 : 0x7fffffff;
 #pragma unroll
-          for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(s[n][e] - m[n][e & 1], z[n][e] - M[n][e & 1]));
-        if (__any_sync(0xffffffffu, top > SLACK)) {
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                  const int kp = e < 2 ? kp0 : kp1, q = pos[n][e & 1];
+                  if (kp > q || (a.window > 0 && kp <= q - a.window)) s[G][n][e] = -INFINITY;
+                }
+            }
+          }
+          // (a bound for the weights: the column's largest score under the tile's largest value scale)
+          const float most = s_most[st];
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float top = fmaxf(s[n][e], s[n][e + 2]), topz = fmaxf(z[n][e], z[n][e + 2]);
+              float x = fmaxf(s[0][n][e], s[0][n][e + 2]);
 #pragma unroll
-              for (int d = 4; d < 32; d <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                topz = fmaxf(topz, __shfl_xor_sync(0xffffffffu, topz, d));
+              for (int G = 1; G < GROUPS; G++) x = fmaxf(x, fmaxf(s[G][n][e], s[G][n][e + 2]));
+              top = fmaxf(top, fmaxf(x - m[n][e], x + most - M[n][e]));
+            }
+          if (__any_sync(0xffffffffu, top > SLACK)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                float m2 = m[n][e], M2 = M[n][e];
+#pragma unroll
+                for (int G = 0; G < GROUPS; G++) {
+                  m2 = fmaxf(m2, fmaxf(s[G][n][e], s[G][n][e + 2]));
+                  M2 = fmaxf(M2, fmaxf(s[G][n][e] + __log2f(sv[G][0]), s[G][n][e + 2] + __log2f(sv[G][1])));
+                }
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                  m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, d));
+                  M2 = fmaxf(M2, __shfl_xor_sync(0xffffffffu, M2, d));
+                }
+                l[n][e] *= ex2(m[n][e] - m2);
+                const float f = ex2(M[n][e] - M2);
+#pragma unroll
+                for (int k = 0; k < DTILES; k++) {
+                  o[k][n][e] *= f;
+                  o[k][n][e + 2] *= f;
+                }
+                m[n][e] = m2;
+                M[n][e] = M2;
+                to_M[n][e] = M2 == LOWEST ? 0.f : ex2(m2 - M2);  // (value scales of zero so far: no weights)
               }
-              // (references are numbers: a column that has seen nothing yet keeps the lowest)
-              const float m2 = fmaxf(m[n][e], top), M2 = fmaxf(M[n][e], topz);
-              l[n][e] *= ex2(m[n][e] - m2);
-              const float f = ex2(M[n][e] - M2);
+          }
+#pragma unroll
+          for (int G = 0; G < GROUPS; G++) {
+            uint32_t b0[WP][NT], b1[WP][NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              float wt[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const float p = ex2(s[G][n][e] - m[n][e & 1]);
+                l[n][e & 1] += p;
+                wt[e] = p * (sv[G][e >> 1] * to_M[n][e & 1]);
+              }
+              if (masked) {  // (the scale of a value that a column does not see may be anything)
+#pragma unroll
+                for (int e = 0; e < 4; e++) wt[e] = s[G][n][e] == -INFINITY ? 0.f : wt[e];
+              }
+              const uint32_t h0 = pack_half(wt[0], wt[1]), h1 = pack_half(wt[2], wt[3]);
+              b0[0][n] = transpose8x8(h0);
+              b1[0][n] = transpose8x8(h1);
+              if (WP == 2) {
+                b0[WP - 1][n] = transpose8x8(rest_half(h0, wt[0], wt[1]));
+                b1[WP - 1][n] = transpose8x8(rest_half(h1, wt[2], wt[3]));
+              }
+            }
+            // O^T: lane group g holds numbers g * HD / 8 and on of the keys in rows 2c, 2c + 1, 2c + 8, 2c + 9
+            constexpr int W = HD / 8;
+            const int r0 = G * 16 + key_of_row(2 * c), r1 = G * 16 + key_of_row(2 * c + 1);
+            auto with_pair = [&](int k, uint32_t lo01, uint32_t hi01) {
+              // lo01: two numbers of the keys in rows 2c and 2c + 1 (bytes: number 0, number 1 of the one, then of the other)
+              const uint32_t a0 = halves(lo01), a1 = halves(lo01 >> 8), a2 = halves(hi01), a3 = halves(hi01 >> 8);
+#pragma unroll
+              for (int p = 0; p < WP; p++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) mma(o[k][n], a0, a1, a2, a3, b0[p][n], b1[p][n]);
+            };
+            if constexpr (W % 4 == 0) {
+              uint32_t v[4][W / 4];
+              constexpr int VEC = W % 16 == 0 ? 16 : W % 8 == 0 ? 8 : 4;  // bytes a read
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int r = (i & 1 ? r1 : r0) + (i >> 1) * 8;
+#pragma unroll
+                for (int u = 0; u < W / VEC; u++) {
+                  const int at = g * W + u * VEC;
+                  const unsigned char* src = vt + place(r, at, swz);
+                  if constexpr (VEC == 16) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src);
+                    v[i][4 * u] = y.x, v[i][4 * u + 1] = y.y, v[i][4 * u + 2] = y.z, v[i][4 * u + 3] = y.w;
+                  } else if constexpr (VEC == 8) {
+                    const uint2 y = *reinterpret_cast<const uint2*>(src);
+                    v[i][2 * u] = y.x, v[i][2 * u + 1] = y.y;
+                  } else {
+                    v[i][u] = *reinterpret_cast<const uint32_t*>(src);
+                  }
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < W / 4; u++) {
+                with_pair(2 * u, __byte_perm(v[0][u], v[1][u], 0x5410), __byte_perm(v[2][u], v[3][u], 0x5410));
+                with_pair(2 * u + 1, __byte_perm(v[0][u], v[1][u], 0x7632), __byte_perm(v[2][u], v[3][u], 0x7632));
+              }
+            } else {
 #pragma unroll
               for (int k = 0; k < DTILES; k++) {
-                o[k][n][e] *= f;
-                o[k][n][e + 2] *= f;
-              }
-              m[n][e] = m2;
-              M[n][e] = M2;
-            }
-        }
-        uint32_t b0[WP][NT], b1[WP][NT];
+                uint32_t v[4];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float wt[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            l[n][e & 1] += ex2(s[n][e] - m[n][e & 1]);
-            wt[e] = ex2(z[n][e] - M[n][e & 1]);
-          }
-          const uint32_t h0 = pack_half(wt[0], wt[1]), h1 = pack_half(wt[2], wt[3]);
-          b0[0][n] = transpose8x8(h0);
-          b1[0][n] = transpose8x8(h1);
-          if (WP == 2) {
-            b0[WP - 1][n] = transpose8x8(rest_half(h0, wt[0], wt[1]));
-            b1[WP - 1][n] = transpose8x8(rest_half(h1, wt[2], wt[3]));
-          }
-        }
-        // O^T: lane group g holds numbers g * HD / 8 and on of the keys in rows 2c, 2c + 1, 2c + 8, 2c + 9
-        constexpr int W = HD / 8;
-        const int r0 = warp * 16 + key_of_row(2 * c), r1 = warp * 16 + key_of_row(2 * c + 1);
-        auto with_pair = [&](int k, uint32_t lo01, uint32_t hi01) {
-          // lo01: two numbers of the keys in rows 2c and 2c + 1 (bytes: number 0, number 1 of the one, then of the other)
-          const uint32_t a0 = halves(lo01), a1 = halves(lo01 >> 8), a2 = halves(hi01), a3 = halves(hi01 >> 8);
-#pragma unroll
-          for (int p = 0; p < WP; p++)
-#pragma unroll
-            for (int n = 0; n < NT; n++) mma(o[k][n], a0, a1, a2, a3, b0[p][n], b1[p][n]);
-        };
-        if constexpr (W % 4 == 0) {
-          uint32_t v[4][W / 4];
-          constexpr int VEC = W % 16 == 0 ? 16 : W % 8 == 0 ? 8 : 4;  // bytes a read
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int r = (i & 1 ? r1 : r0) + (i >> 1) * 8;
-#pragma unroll
-            for (int u = 0; u < W / VEC; u++) {
-              const int at = g * W + u * VEC;
-              const int x = !swz ? 0 : HD == 128 ? r & 7 : (r >> 1) & 3;
-              const unsigned char* src = vt + r * HD + ((((at >> 4) ^ x) << 4) | (at & 15));
-              if constexpr (VEC == 16) {
-                const uint4 y = *reinterpret_cast<const uint4*>(src);
-                v[i][4 * u] = y.x, v[i][4 * u + 1] = y.y, v[i][4 * u + 2] = y.z, v[i][4 * u + 3] = y.w;
-              } else if constexpr (VEC == 8) {
-                const uint2 y = *reinterpret_cast<const uint2*>(src);
-                v[i][2 * u] = y.x, v[i][2 * u + 1] = y.y;
-              } else {
-                v[i][u] = *reinterpret_cast<const uint32_t*>(src);
+                for (int i = 0; i < 4; i++)
+                  v[i] = *reinterpret_cast<const uint16_t*>(vt + ((i & 1 ? r1 : r0) + (i >> 1) * 8) * HD + g * W + 2 * k);
+                with_pair(k, v[0] | v[1] << 16, v[2] | v[3] << 16);
               }
             }
-          }
-#pragma unroll
-          for (int u = 0; u < W / 4; u++) {
-            with_pair(2 * u, __byte_perm(v[0][u], v[1][u], 0x5410), __byte_perm(v[2][u], v[3][u], 0x5410));
-            with_pair(2 * u + 1, __byte_perm(v[0][u], v[1][u], 0x7632), __byte_perm(v[2][u], v[3][u], 0x7632));
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < DTILES; k++) {
-            uint32_t v[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              v[i] = *reinterpret_cast<const uint16_t*>(vt + ((i & 1 ? r1 : r0) + (i >> 1) * 8) * HD + g * W + 2 * k);
-            with_pair(k, v[0] | v[1] << 16, v[2] | v[3] << 16);
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }
       if (!ok) failed = 1;
+      Walk next = w;
+      next.template next_item<L>(a);
+      if (more(next)) load_queries(next);  // on their way while this item's results are put together
 
       // ---------------- the four warps together
 #pragma unroll
@@ -638,157 +855,143 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           for (int i = 1; i < WARPS; i++) top = fmaxf(top, s_M[i][j]);
           f[n][e] = ex2(M[n][e] - top);
         }
+      // s_out[((2 k + h) * 8 + g) * COLS + column]: number g * HD / 8 + 2 k + h, which a lane's row g (h = 0) or g + 8 (h = 1) of
+      // tile k of O^T is.  Two columns a lane next to one another, no bank twice.
+      float2* mine = reinterpret_cast<float2*>(s_out) + g * (COLS / 2) + c;
       for (int turn = 0; turn < WARPS; turn++) {
         if (warp == turn) {
 #pragma unroll
-          for (int k = 0; k < DTILES; k++)
+          for (int k0 = 0; k0 < DTILES; k0 += 4) {  // (reads before writes: four tiles at a time)
+            float2 x[4][NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int k = 0; k < 4; k++)
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                // row (of O^T) g of tile k is number g * HD / 8 + 2 k, row g + 8 the one behind it
-                float* dst = s_out + (n * 8 + 2 * c + (e & 1)) * (HD + 4) + g * (HD / 8) + 2 * k + (e >> 1);
-                const float x = o[k][n][e] * f[n][e & 1];
-                *dst = turn == 0 ? x : *dst + x;
-              }
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                  x[k][n][h] = turn == 0 || k0 + k >= DTILES ? make_float2(0.f, 0.f) : mine[(2 * (k0 + k) + h) * 4 * COLS + n * 4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                  if (k0 + k < DTILES) {
+                    x[k][n][h].x += o[k0 + k][n][2 * h] * f[n][0];
+                    x[k][n][h].y += o[k0 + k][n][2 * h + 1] * f[n][1];
+                    mine[(2 * (k0 + k) + h) * 4 * COLS + n * 4] = x[k][n][h];
+                  }
+          }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
-      const bool all = w.tile == 0 && w.tile_end == w.r.tiles;  // the share holds the item whole
-      for (int j = warp; j < COLS; j += WARPS) {
-        float top = s_m[0][j], topM = s_M[0][j], sum = 0.f;
+      // a lane a column: the references and sums of the four warps
+      float top = LOWEST, topM = LOWEST, sum = 0.f;
+      {
+        const int j = lane % COLS;
 #pragma unroll
-        for (int i = 1; i < WARPS; i++) {
+        for (int i = 0; i < WARPS; i++) {
           top = fmaxf(top, s_m[i][j]);
           topM = fmaxf(topM, s_M[i][j]);
         }
 #pragma unroll
         for (int i = 0; i < WARPS; i++) sum += s_l[i][j] * ex2(s_m[i][j] - top);
-        const float* src = s_out + j * (HD + 4);
-        if (all) {
-          if (col0 + j < cols) {
-            T* dst = reinterpret_cast<T*>(a.out) + (a.q_start[w.r.s] + (col0 + j) / a.group) * a.out_stride +
-                     (long long)(kvh * a.group + (col0 + j) % a.group) * HD;
-            const float r = last_factor(topM, top, sum);
-            for (int d = lane; d < HD; d += 32) dst[d] = from_float<T>(src[d] * r);
-          }
-        } else {
-          float* dst = a.parts + ((((long long)kvh * gridDim.x + blockIdx.x) * 2 + (w.opens ? 0 : 1)) * COLS + j) * (HD + 4);
-          for (int d = lane; d < HD; d += 32) dst[d] = src[d];
-          if (lane == 0) {
-            dst[HD] = topM;
-            dst[HD + 1] = top;
-            dst[HD + 2] = sum;
-          }
+      }
+      if (holds_whole(w)) {
+        const float factor = last_factor(topM, top, sum);  // (of column lane % COLS)
+        for (int i = threadIdx.x; i < COLS * 8; i += 128) store_run<T, COLS>(a.out, s_out, w.r.q_start, col0, cols, i, factor, kvh);
+      } else {
+        float* dst = a.parts + (((long long)kvh * gridDim.x + blockIdx.x) * 2 + (w.opens ? 0 : 1)) * L::PART;
+        for (int i = threadIdx.x; i < COLS * HD / 4; i += 128) reinterpret_cast<float4*>(dst)[i] = reinterpret_cast<const float4*>(s_out)[i];
+        if (warp == 0 && lane < COLS) {
+          dst[COLS * HD + lane] = topM;
+          dst[COLS * HD + COLS + lane] = top;
+          dst[COLS * HD + 2 * COLS + lane] = sum;
         }
       }
+      w = next;
+    }
+    // ---------------- items that this share holds a part of, at most two: whoever left an item's last part puts it together
+    // (behind the loop, which has no registers to spare)
+    float (*s_fac)[COLS] = reinterpret_cast<float(*)[COLS]>(ring);  // (every tile that was asked for has been used)
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (threadIdx.x == 0 && (s_cut[0].n > 0 || s_cut[1].n > 0)) {
+      __threadfence();  // (for all of the block's: the barrier stands between their stores and this)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (s_cut[i].n > 0 && !arrive(a.arrived + (long long)kvh * gridDim.x + s_cut[i].b0, s_cut[i].n)) s_cut[i].n = 0;
+      __threadfence();
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+      const CutItem x = s_cut[i];
+      if (x.n == 0) continue;
+      // of the first share its first item or its last, of the others the first
+      const float* rest = a.parts + ((long long)kvh * gridDim.x + x.b0) * 2 * L::PART;
+      join_parts<T, NT>(a.out, rest + (shares.start(x.b0) >= x.at ? 0 : L::PART), rest, x.n, s_out, s_fac, x.q_start, x.col0, x.cols, kvh);
     }
   }
   __syncthreads();
   if (threadIdx.x == 0 && failed) atomicOr(a.status, TKB_STATUS_WAIT_TIMEOUT);
 }
 
-// The parts of items that no share holds whole, in the order of the shares.  A block a request and kv head, a warp a column.
-template <typename T, int NT>
-__global__ void __launch_bounds__(128) attn_kv8_join_kernel(const Args a, int blocks) {
-  constexpr int COLS = 8 * NT;
-  trigger_dependents();
-  grid_dependency_wait();
-  Request r;
-  const int total = a.base[a.n_seqs], base = a.base[blockIdx.x];
-  if (!r.load(a, blockIdx.x, COLS)) return;
-  const Shares shares(total, blocks);
-  const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int ct = 0; ct < r.col_tiles; ct++) {
-    const int at = base + ct * r.tiles, b0 = shares.of(at), b1 = shares.of(at + r.tiles - 1);
-    if (b0 == b1) continue;
-    // the share's first item, or its last
-    const float* first = a.parts + (((long long)kvh * blocks + b0) * 2 + (shares.start(b0) >= at ? 0 : 1)) * COLS * (HD + 4);
-    const float* rest = a.parts + ((long long)kvh * blocks + b0 + 1) * 2 * COLS * (HD + 4);
-    const int n = b1 - b0 + 1;
-    for (int j = warp; j < COLS && ct * COLS + j < r.q_len * a.group; j += 4) {
-      auto part = [&](int i) { return (i == 0 ? first : rest + (long long)(i - 1) * 2 * COLS * (HD + 4)) + j * (HD + 4); };
-      float top = LOWEST, topM = LOWEST;
-      for (int i = lane; i < n; i += 32) {
-        const float* p = part(i);
-        topM = fmaxf(topM, p[HD]);
-        top = fmaxf(top, p[HD + 1]);
-      }
-      top = warp_max(top);
-      topM = warp_max(topM);
-      float sum = 0.f, acc[(HD + 31) / 32];
-#pragma unroll
-      for (int i = 0; i < (HD + 31) / 32; i++) acc[i] = 0.f;
-#pragma unroll 4
-      for (int b = 0; b < n; b++) {
-        const float* p = part(b);
-        sum += p[HD + 2] * ex2(p[HD + 1] - top);
-        const float f = ex2(p[HD] - topM);
-#pragma unroll
-        for (int i = 0; i < (HD + 31) / 32; i++)
-          if (lane + 32 * i < HD) acc[i] += p[lane + 32 * i] * f;
-      }
-      const float f = last_factor(topM, top, sum);
-      const int col = ct * COLS + j;
-      T* dst = reinterpret_cast<T*>(a.out) + (a.q_start[r.s] + col / a.group) * a.out_stride + (long long)(kvh * a.group + col % a.group) * HD;
-#pragma unroll
-      for (int i = 0; i < (HD + 31) / 32; i++)
-        if (lane + 32 * i < HD) dst[lane + 32 * i] = from_float<T>(acc[i] * f);
-    }
-  }
-}
-
+// The codes of all pages as rows of 128 bytes.
 int make_map_codes(CUtensorMap* map, const void* base, long long rows, int box_rows) {
-  cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)HD};
-  cuuint32_t box[2] = {(cuuint32_t)HD, (cuuint32_t)box_rows};
+  cuuint64_t dims[2] = {128, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {128};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
 }
 
-// How many blocks a kv head gets, and whether shares are whole items.  Both from bounds: `col_tiles` items of at most `tiles`.
+// The scratch: counts of parts, then the parts.
+long long arrived_bytes(int nkv, int blocks) { return ((long long)nkv * blocks + 1) / 2 * 16; }
+
+// How many blocks a kv head gets, and whether shares are whole items.  Both from bounds: `col_tiles` items of keys up to `max_kv`.
 struct Cut {
   int blocks, whole;
 };
-Cut cut(int col_tiles, int tiles, int nkv) {
-  const int slots = sm_count() * (HD <= 64 ? 4 : HD <= 128 ? 3 : 1) / nkv;
+template <typename L> Cut cut(int col_tiles, int max_kv, int nkv) {
+  const int tiles = (max_kv + L::BKV - 1) / L::BKV + 1;  // (a window's first tile starts before it)
+  const int slots = sm_count() * L::BLOCKS / nkv;
   Cut c;
-  const long long total = (long long)col_tiles * tiles;
-  c.whole = tiles <= 4;
-  long long b = c.whole ? col_tiles : total / 2;  // two tiles a share at least
+  c.whole = max_kv <= WHOLE_KEYS;
+  long long b = c.whole ? col_tiles : (long long)col_tiles * tiles;
   if (b > slots) b = slots;
+  if (b > 1022) b = 1022;  // (a count of parts has ten bits)
   c.blocks = b < 1 ? 1 : (int)b;
   return c;
 }
 
 template <typename T, int NT>
-int launch(Args a, int col_tiles, int tiles, cudaStream_t st) {
-  constexpr int BYTES = Layout<T, NT>::BYTES;
+int launch(Args a, int col_tiles, int max_kv, cudaStream_t st) {
+  using L = Layout<T, NT>;
+  constexpr int BYTES = L::BYTES;
   static SharedMemoryRequest ask;
   int rc = ask({{(const void*)attn_kv8_kernel<T, NT>, BYTES}});
   if (rc) return rc;
   CUtensorMap map_k, map_v;
   memset(&map_k, 0, sizeof(map_k));
   memset(&map_v, 0, sizeof(map_v));
-  const long long rows = (long long)a.num_pages * a.nkv * a.ps;
+  const long long rows = (long long)a.num_pages * a.nkv * a.ps * HD / 128;
   a.tma_rows = 0;
   if (SWIZZLES && a.ps_shift >= 3 && rows < (1ll << 31)) {
-    a.tma_rows = a.ps < BKV ? a.ps : BKV;
+    a.tma_rows = (a.ps < L::BKV ? a.ps : L::BKV) * HD / 128;  // a page's, or a tile's of a larger page
     if ((rc = get_encode()) || (rc = make_map_codes(&map_k, a.kcache, rows, a.tma_rows)) || (rc = make_map_codes(&map_v, a.vcache, rows, a.tma_rows)))
       return rc;
   }
-  const Cut c = cut(col_tiles, tiles, a.nkv);
+  if ((long long)col_tiles * (max_kv / L::BKV + 2) > 0x7fffffffll) return -3;
+  const Cut c = cut<L>(col_tiles, max_kv, a.nkv);
   a.whole = c.whole;
-  rc = launch_pdl(attn_kv8_kernel<T, NT>, dim3(c.blocks, a.nkv), dim3(THREADS), (size_t)BYTES, st, map_k, map_v, a);
-  if (rc || c.whole) return rc;
-  return launch_pdl(attn_kv8_join_kernel<T, NT>, dim3(a.n_seqs, a.nkv), dim3(128), 0, st, a, c.blocks);
+  a.parts = (float*)((char*)a.arrived + arrived_bytes(a.nkv, c.blocks));
+  static std::atomic<unsigned long long> launches{(unsigned long long)std::chrono::system_clock::now().time_since_epoch().count() << 16};
+  a.tag = launches.fetch_add(1, std::memory_order_relaxed) & ((1ull << 54) - 1);
+  return launch_pdl(attn_kv8_kernel<T, NT>, dim3(c.blocks, a.nkv), dim3(THREADS), (size_t)BYTES, st, map_k, map_v, a);
 }
-
-// where the parts start in the scratch
-long long parts_at(int n_seqs) { return ((long long)n_seqs + 1 + 3) / 4 * 16; }
 
 // column tiles of all requests, at most, when a block takes `cols` of them
 int most_col_tiles(int n_seqs, int singles, int tokens, int group, int cols) {
@@ -800,13 +1003,15 @@ int most_col_tiles(int n_seqs, int singles, int tokens, int group, int cols) {
 
 // Bytes of scratch that tkb_attn_kv8 wants with the same sizes.
 TKB_EXPORT long long tkb_attn_kv8_scratch(int n_seqs, int singles, int tokens, int max_kv, int nkv, int group) {
-  long long most = 0;
-  for (int nt = 1; nt <= max_nt(); nt++) {
-    const Cut c = cut(most_col_tiles(n_seqs, singles, tokens, group, 8 * nt), (max_kv + BKV - 1) / BKV + 1, nkv);
-    const long long n = (long long)nkv * c.blocks * 2 * 8 * nt * (HD + 4) * 4;
+  if (n_seqs <= 0 || nkv <= 0 || group <= 0 || max_kv <= WHOLE_KEYS) return 0;
+  const Cut one = cut<Layout<float, 1>>(most_col_tiles(n_seqs, singles, tokens, group, 8), max_kv, nkv);
+  long long most = arrived_bytes(nkv, one.blocks) + (long long)nkv * one.blocks * 2 * Layout<float, 1>::PART * 4;
+  if constexpr (max_nt() == 2) {
+    const Cut two = cut<Layout<float, 2>>(most_col_tiles(n_seqs, singles, tokens, group, 16), max_kv, nkv);
+    const long long n = arrived_bytes(nkv, two.blocks) + (long long)nkv * two.blocks * 2 * Layout<float, 2>::PART * 4;
     if (n > most) most = n;
   }
-  return most + parts_at(n_seqs);
+  return most;
 }
 
 // q, out: rows of heads (f32 != 0: float32, else bfloat16).  singles: requests that bring one token; tokens: rows of q;
@@ -819,22 +1024,22 @@ TKB_EXPORT int tkb_attn_kv8(const void* q, long long q_stride, void* out, long l
   if (nkv <= 0 || nh <= 0 || nh % nkv || ps <= 0 || window < 0 || singles < 0 || singles > n_seqs || singles > tokens || max_kv < 0) return -2;
   if (nkv > 65535) return -3;
   Args a = {};
-  a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.q = q, a.q_stride = q_stride;
+  a.out.rows = out, a.out.stride = out_stride, a.out.group = nh / nkv, a.out.mul = (unsigned)(0xffffffffu / (unsigned)a.out.group) + 1u;
   a.kcache = (const int8_t*)kcache, a.vcache = (const int8_t*)vcache, a.k_scale = k_scale, a.v_scale = v_scale;
   a.q_start = q_start, a.q_len = q_len, a.kv_len = kv_len, a.page_indptr = page_indptr, a.page_ids = page_ids;
-  a.base = (int*)scratch;
-  a.parts = (float*)((char*)scratch + parts_at(n_seqs));
-  a.n_seqs = n_seqs, a.group = nh / nkv, a.nkv = nkv, a.ps = ps, a.window = window, a.num_pages = num_pages, a.status = status;
+  a.arrived = (unsigned long long*)scratch;
+  a.n_seqs = n_seqs, a.nkv = nkv, a.ps = ps, a.window = window, a.num_pages = num_pages, a.status = status;
   a.ps_shift = (ps & (ps - 1)) == 0 ? 31 - __builtin_clz(ps) : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.which = SINGLE | PORTION;
   cudaStream_t st = (cudaStream_t)st_;
-  // one tile of 8 columns for single tokens of up to 8 heads a kv head, two where there are more columns to fill them
-  const int nt = max_nt() == 2 && (singles < n_seqs || a.group > 8) ? 2 : 1;
-  const int col_tiles = most_col_tiles(n_seqs, singles, tokens, a.group, 8 * nt), tiles = (max_kv + BKV - 1) / BKV + 1;
-  if ((long long)col_tiles * tiles > 0x7fffffffll) return -3;
+  // one tile of 8 columns for single tokens of up to 8 heads a kv head, two where there are more columns to fill them (and for
+  // pages of one token, of which a tile of 128 keys has more than a window holds)
+  const int nt = max_nt() == 2 && (singles < n_seqs || a.out.group > 8 || ps == 1) ? 2 : 1;
+  const int col_tiles = most_col_tiles(n_seqs, singles, tokens, a.out.group, 8 * nt);
   if constexpr (max_nt() == 2) {
-    if (nt == 2) return f32 ? launch<float, 2>(a, col_tiles, tiles, st) : launch<bf16, 2>(a, col_tiles, tiles, st);
+    if (nt == 2) return f32 ? launch<float, 2>(a, col_tiles, max_kv, st) : launch<bf16, 2>(a, col_tiles, max_kv, st);
   }
-  return f32 ? launch<float, 1>(a, col_tiles, tiles, st) : launch<bf16, 1>(a, col_tiles, tiles, st);
+  return f32 ? launch<float, 1>(a, col_tiles, max_kv, st) : launch<bf16, 1>(a, col_tiles, max_kv, st);
 }
