@@ -57,8 +57,9 @@ template <typename T, int NT> struct Layout {
   static constexpr int GROUPS = NT == 1 && HD <= 128 ? 2 : 1;
   static constexpr int BKV = 16 * GROUPS * WARPS;  // keys a tile
   static constexpr int KV_BYTES = BKV * HD;
-  static constexpr int STAGES = HD <= 64 ? 8 / GROUPS : HD <= 128 ? 4 / GROUPS : 2;
-  static constexpr int BLOCKS = HD > 128 ? 1 : NT == 2 ? 2 : 3;  // blocks an SM
+  static constexpr int STAGES = HD <= 64 ? 8 / GROUPS : HD <= 128 ? 6 / GROUPS : 2;
+  // blocks an SM (heads of 128 with three, of 128 registers: 64 requests of 8,192 keys 195 us, one of 60,000 47; with two 184 and 38)
+  static constexpr int BLOCKS = HD > 128 ? 1 : NT == 2 || HD > 64 ? 2 : 3;
   static constexpr int QP = sizeof(T) == 4 ? 3 : 2;  // pieces of a query
   static constexpr int WP = sizeof(T) == 4 ? 2 : 1;  // pieces of a weight
   static constexpr int COLS = 8 * NT;
@@ -1001,7 +1002,7 @@ int most_col_tiles(int n_seqs, int singles, int tokens, int group, int cols) {
 
 }  // namespace
 
-// Bytes of scratch that tkb_attn_kv8 wants with the same sizes.
+// Bytes of scratch that tkb_attn_kv8 wants with the same sizes (n_seqs, tokens: both `singles` where it is to take those only).
 TKB_EXPORT long long tkb_attn_kv8_scratch(int n_seqs, int singles, int tokens, int max_kv, int nkv, int group) {
   if (n_seqs <= 0 || nkv <= 0 || group <= 0 || max_kv <= WHOLE_KEYS) return 0;
   const Cut one = cut<Layout<float, 1>>(most_col_tiles(n_seqs, singles, tokens, group, 8), max_kv, nkv);
@@ -1015,13 +1016,13 @@ TKB_EXPORT long long tkb_attn_kv8_scratch(int n_seqs, int singles, int tokens, i
 }
 
 // q, out: rows of heads (f32 != 0: float32, else bfloat16).  singles: requests that bring one token; tokens: rows of q;
-// max_kv: no request has more keys.  scratch: see above, on a 16-byte boundary.
+// max_kv: no request has more keys.  which: 1 the requests that bring one token, 2 the others, 3 all.  scratch: see above, on a 16-byte boundary.
 TKB_EXPORT int tkb_attn_kv8(const void* q, long long q_stride, void* out, long long out_stride, int f32, const void* kcache,
                             const void* vcache, const float* k_scale, const float* v_scale, const int* q_start, const int* q_len,
                             const int* kv_len, const int* page_indptr, const int* page_ids, void* scratch, int n_seqs, int singles, int tokens,
-                            int max_kv, int nh, int nkv, int ps, float scale, int window, int num_pages, int* status, void* st_) {
-  if (n_seqs <= 0 || tokens <= 0) return 0;
-  if (nkv <= 0 || nh <= 0 || nh % nkv || ps <= 0 || window < 0 || singles < 0 || singles > n_seqs || singles > tokens || max_kv < 0) return -2;
+                            int max_kv, int nh, int nkv, int ps, float scale, int window, int num_pages, int which, int* status, void* st_) {
+  if (n_seqs <= 0 || tokens <= 0 || (which == SINGLE && singles == 0)) return 0;
+  if (nkv <= 0 || nh <= 0 || nh % nkv || ps <= 0 || window < 0 || singles < 0 || singles > n_seqs || singles > tokens || max_kv < 0 || which < 1 || which > 3) return -2;
   if (nkv > 65535) return -3;
   Args a = {};
   a.q = q, a.q_stride = q_stride;
@@ -1032,12 +1033,14 @@ TKB_EXPORT int tkb_attn_kv8(const void* q, long long q_stride, void* out, long l
   a.n_seqs = n_seqs, a.nkv = nkv, a.ps = ps, a.window = window, a.num_pages = num_pages, a.status = status;
   a.ps_shift = (ps & (ps - 1)) == 0 ? 31 - __builtin_clz(ps) : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.which = SINGLE | PORTION;
+  a.which = which;
   cudaStream_t st = (cudaStream_t)st_;
   // one tile of 8 columns for single tokens of up to 8 heads a kv head, two where there are more columns to fill them (and for
   // pages of one token, of which a tile of 128 keys has more than a window holds)
-  const int nt = max_nt() == 2 && (singles < n_seqs || a.out.group > 8 || ps == 1) ? 2 : 1;
-  const int col_tiles = most_col_tiles(n_seqs, singles, tokens, a.out.group, 8 * nt);
+  if (which == SINGLE) tokens = singles;
+  const int counted = which == SINGLE ? singles : n_seqs;
+  const int nt = max_nt() == 2 && (singles < counted || a.out.group > 8 || ps == 1) ? 2 : 1;
+  const int col_tiles = most_col_tiles(counted, singles, tokens, a.out.group, 8 * nt);
   if constexpr (max_nt() == 2) {
     if (nt == 2) return f32 ? launch<float, 2>(a, col_tiles, max_kv, st) : launch<bf16, 2>(a, col_tiles, max_kv, st);
   }

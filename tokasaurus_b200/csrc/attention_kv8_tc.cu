@@ -1,0 +1,700 @@
+// Causal grouped-query attention of prompt portions over a cache held in 8 bits (cache8.cu) on the fifth-generation tensor
+// cores; compile with -DTKB_HD (a multiple of 16 to 128).  Formulas as in attention_kv8.cu.
+//
+// The (token, head) pairs of one request and kv head are ROWS.  A block owns 256 of them in two units of 128 and walks the keys
+// they may see in tiles of 64, which are brought once for both; where that would leave SMs without a block it owns 128, and
+// the units take every second tile each and are put together at the end.
+//     converters  four warps, two threads a key: codes from the cache into registers (the tile behind is on its way meanwhile),
+//                 made halves exactly, and into a ring of K and V tiles in the tensor cores' swizzled layout; each key's scales
+//                 beside them.  Values' scales are brought under the largest that the item sees (a power of two), so that
+//                 weights fit half precision
+//     MMA         a warp a unit:  S = Q K^T (128 x 64 x 16, two S tiles in tensor memory), O += P V (128 x HD x 16) with P from
+//                 tensor memory, O accumulating there over all tiles; V stays [key][head size], an MN-major operand
+//     softmax     four warps a unit, a thread a row: scores into registers, times the keys' scales, row maximum, exponentials and
+//                 sum, times the values' scales, P as halves over the row's own scores
+// The exponentials of a row use a reference that stays put while its scores stay below it + 4 (log2); when a row tops that, its
+// warp scales its rows of O.  Queries are brought to [1, 2) by a power of two a row; in float32 steps Q and P go in as two halves
+// each (22 bits).  Every wait is bounded (TKB_STATUS_WAIT_TIMEOUT).
+#include "tcgen05.cuh"
+#include "per_device.h"
+#include <cuda_fp16.h>
+
+#ifndef TKB_HD
+#error "compile with -DTKB_HD=<head size>"
+#endif
+
+using namespace tkb5;
+
+namespace {
+
+constexpr int HD = TKB_HD;
+static_assert(HD % 16 == 0 && HD >= 16 && HD <= 128, "head size");
+constexpr int ATOMS = (HD + 63) / 64;    // 128-byte blocks of a row
+constexpr int BQ = 128;                  // rows a unit
+constexpr int BKV = 64;                  // keys a tile
+constexpr int UNITS = 2;
+constexpr int SOFTMAX_WARPS = 4 * UNITS, MMA_WARP = SOFTMAX_WARPS, CONVERT_WARP = MMA_WARP + UNITS;
+constexpr int THREADS = (CONVERT_WARP + 4) * 32;
+constexpr int Q_BYTES = ATOMS * BQ * 128;
+constexpr int KV_BYTES = ATOMS * BKV * 128;
+constexpr uint32_t TMEM_COLS = 512;      // a unit: two S (then P) of 64 columns, O behind them
+constexpr float NEG_BIG = -1.0e30f;
+constexpr float REF_SLACK = 4.f;
+
+template <typename T> struct Layout {
+  static constexpr int PIECES = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int Q = UNITS * PIECES * Q_BYTES;
+  static constexpr int STAGES = (200 * 1024 - Q) / (2 * KV_BYTES) < 6 ? (200 * 1024 - Q) / (2 * KV_BYTES) : 6;
+  static constexpr int BYTES = 1024 + Q + STAGES * 2 * KV_BYTES;
+  static_assert(STAGES >= 2 && BQ * HD * 4 <= STAGES * 2 * KV_BYTES, "a unit's output goes through the ring's memory");
+};
+
+struct Args {
+  const void* q;
+  void* out;
+  const int8_t *kcache, *vcache;
+  const float *k_scale, *v_scale;
+  const int *q_start, *q_len, *kv_len, *page_indptr, *page_ids;
+  long long q_stride, out_stride;
+  int n_seqs, group, nkv, ps, ps_shift, window, num_pages, rows;  // rows: of a block (128 or 256)
+  float scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// D += A B with A in tensor memory (row = lane, two neighbouring k's a column), by a whole warp
+__device__ __forceinline__ void umma_a_tmem(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nelect.sync _|q, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// MN-major operand (V as [key][64]): rows of 128 bytes, 8-key groups 1,024 bytes apart, the next 64 numbers a block further
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)((BKV * 128) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// Instruction descriptor: D = float32, A = B = half.
+__host__ __device__ constexpr uint32_t idesc_half(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t rest_half(uint32_t h, float lo, float hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack_half(lo - f.x, hi - f.y);
+}
+// Four codes, their sign bits turned, as two pairs of halves: 0x64cc is 1024 + cc.
+__device__ __forceinline__ void four_halves(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t twice(float x) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t both(uint32_t lo, uint32_t hi) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(lo), "r"(hi));
+  return y;
+}
+__device__ __forceinline__ void split(uint64_t x, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// A row's 32 scores of a half tile times the keys' scales (in place) and their largest.  MASKED: columns outside [lo, lo + span]
+// and those whose bit is missing have none.
+template <bool MASKED>
+__device__ __forceinline__ float scale_max(uint32_t (&s)[32], const float* __restrict__ sk, int lo, uint32_t span, uint32_t there) {
+  float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(sk + i);
+    split(mul2(both(s[i], s[i + 1]), k.x), s[i], s[i + 1]);
+    split(mul2(both(s[i + 2], s[i + 3]), k.y), s[i + 2], s[i + 3]);
+    if (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if ((uint32_t)(i + e - lo) > span || !((there >> (i + e)) & 1)) s[i + e] = 0xff800000u;
+    }
+    m0 = max3(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+    m1 = max3(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+  }
+  return max_nan(m0, m1);
+}
+// p = 2^(s * rs - m) of 32 scores, added to `sum`; w = p * sv as pairs of halves (LOW: and what those leave over).  MASKED: where there
+// is no score the weight is zero whatever the value's scale is.
+template <bool MASKED, bool LOW>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], const float* __restrict__ sv, uint32_t* hi, uint32_t* low, uint64_t rs,
+                                        uint64_t neg_m, uint64_t& sum) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(sv + i);
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      uint32_t x0, x1;
+      split(fma2(both(s[i + e], s[i + e + 1]), rs, neg_m), x0, x1);
+      const float p0 = fast_exp2(__uint_as_float(x0)), p1 = fast_exp2(__uint_as_float(x1));
+      const uint64_t p = both(__float_as_uint(p0), __float_as_uint(p1));
+      sum = add2(sum, p);
+      uint32_t w0, w1;
+      split(mul2(p, e == 0 ? v.x : v.y), w0, w1);
+      if (MASKED) {
+        if (s[i + e] == 0xff800000u) w0 = 0;
+        if (s[i + e + 1] == 0xff800000u) w1 = 0;
+      }
+      const uint32_t h = pack_half(__uint_as_float(w0), __uint_as_float(w1));
+      hi[(i + e) >> 1] = h;
+      if (LOW) low[(i + e) >> 1] = rest_half(h, __uint_as_float(w0), __uint_as_float(w1));
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
+  using L = Layout<T>;
+  constexpr int PIECES = L::PIECES, STAGES = L::STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], s_full[UNITS][2], p_full[UNITS], o_done[UNITS], merged;
+  __shared__ __align__(16) float s_sk[STAGES][BKV], s_sv[STAGES][BKV];
+  __shared__ __align__(8) uint16_t s_there[STAGES][4];
+  __shared__ float unit_m[BQ], unit_l[BQ];
+  __shared__ int s_scan[THREADS / 32], s_item[2];
+  __shared__ unsigned s_top[4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  unsigned char* sQ = base;
+  unsigned char* ring = base + L::Q;  // a stage: K, then V
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  trigger_dependents();
+  if (tid == 0) s_item[0] = -1;
+  grid_dependency_wait();
+  __syncthreads();
+
+  // ---------------- which request and rows: items stand request by request, the last rows (which see the most keys) first
+  const int kvh = blockIdx.x % a.nkv, rank = blockIdx.x / a.nkv;
+  {
+    const int per = (a.n_seqs + THREADS - 1) / THREADS;
+    const int lo = min(a.n_seqs, tid * per), hi = min(a.n_seqs, lo + per);
+    auto items = [&](int s) {
+      const int n = a.q_len[s];
+      return n > 1 ? (n * a.group + a.rows - 1) / a.rows : 0;
+    };
+    int mine = 0;
+    for (int s = lo; s < hi; s++) mine += items(s);
+    int before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    if (lane == 31) s_scan[warp] = before;
+    __syncthreads();
+    before -= mine;
+    for (int i = 0; i < warp; i++) before += s_scan[i];
+    if (rank >= before && rank < before + mine) {
+      int at = before;
+      for (int s = lo; s < hi; s++) {
+        const int n = items(s);
+        if (rank < at + n) {
+          s_item[0] = s;
+          s_item[1] = n - 1 - (rank - at);
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  const int s = s_item[0];
+  if (s < 0) return;
+  const int q_len = a.q_len[s], kv_len = a.kv_len[s], row0 = s_item[1] * a.rows, all_rows = q_len * a.group;
+  const int live_rows = min(a.rows, all_rows - row0);
+  const bool streams = a.rows == BQ;          // the units share the rows and take every second tile each
+  const int p0 = kv_len - q_len;
+  const int first_pos = p0 + row0 / a.group, last_pos = p0 + (row0 + live_rows - 1) / a.group;
+  int k_begin = 0;
+  if (a.window > 0 && first_pos - a.window + 1 > 0) k_begin = (first_pos - a.window + 1) & ~(BKV - 1);
+  const int n_tiles = (last_pos + 1 - k_begin + BKV - 1) / BKV;
+  const int live_units = streams ? (n_tiles > 1 ? 2 : 1) : (live_rows > BQ ? 2 : 1);
+  // tiles of unit u: u, u + step, ... (streams) or all
+  const int step = streams ? 2 : 1;
+  const int* table = a.page_ids + a.page_indptr[s];
+
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], streams ? 1 : live_units);
+    }
+    for (int u = 0; u < UNITS; u++) {
+      mbar_init(&s_full[u][0], 1);
+      mbar_init(&s_full[u][1], 1);
+      mbar_init(&p_full[u], 4);
+      mbar_init(&o_done[u], 1);
+    }
+    mbar_init(&merged, 4);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+
+  // ---------------- queries: a thread its row, to [1, 2) by a power of two, as halves into the swizzled tile
+  const int unit = warp >> 2, r = tid & (BQ - 1);
+  const int urow = streams ? r : unit * BQ + r;  // row of the item (softmax threads)
+  const bool row_live = warp < SOFTMAX_WARPS && unit < live_units && urow < live_rows;
+  const int flat = row0 + min(urow, live_rows - 1);
+  const int token = flat / a.group, head = kvh * a.group + flat - token * a.group;
+  float row_scale = 0.f;
+  if (warp < SOFTMAX_WARPS && unit < live_units && (!streams || unit == 0)) {
+    const T* src = reinterpret_cast<const T*>(a.q) + (a.q_start[s] + token) * a.q_stride + (long long)head * HD;
+    const bool wide = (((uintptr_t)src) & 15) == 0;
+    unsigned top = 0;
+    auto chunk = [&](int c, float (&v)[8]) {  // eight numbers
+      if (!row_live) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = 0.f;
+      } else if (wide) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src + c * 8), y = *reinterpret_cast<const float4*>(src + c * 8 + 4);
+          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + c * 8);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            v[2 * e] = __uint_as_float(w[e] << 16);
+            v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = to_float(src[c * 8 + e]);
+      }
+    };
+#pragma unroll 4
+    for (int c = 0; c < HD / 8; c++) {
+      float v[8];
+      chunk(c, v);
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    }
+    const int e = max(1, (int)(top >> 23)) - 127;
+    const float down = __uint_as_float(e >= 127 ? 0x00400000u : (unsigned)(127 - e) << 23);
+    row_scale = top < 0x7f800000u ? a.scale_log2 * __uint_as_float((unsigned)(127 + e) << 23) : NAN;
+    unsigned char* dst = sQ + unit * PIECES * Q_BYTES + r * 128;
+#pragma unroll 4
+    for (int c = 0; c < HD / 8; c++) {
+      float v[8];
+      chunk(c, v);  // (from the cache)
+      uint32_t h[4], low[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x = top < 0x7f800000u ? v[2 * i] * down : 0.f, y = top < 0x7f800000u ? v[2 * i + 1] * down : 0.f;
+        h[i] = pack_half(x, y);
+        low[i] = rest_half(h[i], x, y);
+      }
+      const int at = (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4);
+      *reinterpret_cast<uint4*>(dst + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (PIECES == 2) *reinterpret_cast<uint4*>(dst + Q_BYTES + at) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+    if (streams) unit_m[r] = row_scale;
+    fence_proxy_async();
+  }
+  // ---------------- the item's largest value scale, as a power of two
+  if (warp >= CONVERT_WARP) {
+    const int t = tid - CONVERT_WARP * 32;
+    const int page0 = (a.window > 0 ? max(0, first_pos - a.window + 1) : 0) / a.ps, page1 = last_pos / a.ps;  // pages that are seen
+    unsigned top = 0;
+    for (int p = page0 + t; p <= page1; p += 128) {
+      bool bad = false;
+      const int page = checked_page(__ldg(table + p), a.num_pages, bad);
+      if (page >= 0) {
+        const unsigned v = __float_as_uint(a.v_scale[(long long)page * a.nkv + kvh]);
+        if (v < 0x7f800000u) top = max(top, v);
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_top[warp - CONVERT_WARP] = top;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // 2^(10 - e) with e the exponent of the largest: the scaled ones are below 2^11, a weight below 2^15
+  const int v_exp = min(max((int)(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])) >> 23) - 127, -110), 127);
+
+  if (warp >= CONVERT_WARP) {
+    // ---------------- converters
+    const int t = tid - CONVERT_WARP * 32, key = t >> 1, half = t & 1;
+    constexpr int PAIRS = ATOMS * 2;  // 16 codes each: two 16-byte chunks of the tile's row
+    const float down = __uint_as_float((unsigned)(127 + 10 - v_exp) << 23);
+    bool ok = true, bad = false;
+    auto page_of = [&](int j) {
+      const int k = k_begin + j * BKV + key;
+      if (j >= n_tiles || k > last_pos) return -1;
+      return __ldg(table + (a.ps_shift >= 0 ? k >> a.ps_shift : k / a.ps));
+    };
+    uint4 kc[PAIRS], vc[PAIRS];
+    float scale = 0.f;
+    int page = -1;
+    auto fetch = [&](int j, int id) {
+      page = checked_page(id, a.num_pages, bad);
+      const int k = k_begin + j * BKV + key;
+      const int slot = a.ps_shift >= 0 ? k & (a.ps - 1) : k % a.ps;
+      const long long block = (long long)max(page, 0) * a.nkv + kvh;
+      const int8_t* ks = a.kcache + (block * a.ps + slot) * HD;
+      const int8_t* vs = a.vcache + (block * a.ps + slot) * HD;
+      scale = page >= 0 ? (half ? a.v_scale : a.k_scale)[block] : 0.f;
+#pragma unroll
+      for (int i = 0; i < PAIRS; i++) {
+        const int c = (i >> 1) * 8 + half * 4 + (i & 1) * 2;
+        kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
+        if (page >= 0 && c < HD / 8) {
+          kc[i] = __ldg(reinterpret_cast<const uint4*>(ks + c * 8));
+          vc[i] = __ldg(reinterpret_cast<const uint4*>(vs + c * 8));
+        }
+      }
+    };
+    fetch(0, page_of(0));
+    int next_id = page_of(1);
+    for (int j = 0; j < n_tiles; j++) {
+      const int st = j % STAGES;
+      if (j >= STAGES && !mbar_wait_idle(&empty[st], ((j / STAGES) - 1) & 1)) { ok = false; break; }
+      unsigned char* dk = ring + st * 2 * KV_BYTES + key * 128;
+#pragma unroll
+      for (int i = 0; i < PAIRS; i++) {
+        const int c = (i >> 1) * 8 + half * 4 + (i & 1) * 2;
+        if (c < HD / 8) {
+          unsigned char* d0 = dk + (c >> 3) * (BKV * 128);
+#pragma unroll
+          for (int w = 0; w < 2; w++) {
+            const int at = (((c + w) & 7) ^ (key & 7)) << 4;
+            uint4 x;
+            four_halves(w ? kc[i].z : kc[i].x, x.x, x.y);
+            four_halves(w ? kc[i].w : kc[i].y, x.z, x.w);
+            *reinterpret_cast<uint4*>(d0 + at) = x;
+            four_halves(w ? vc[i].z : vc[i].x, x.x, x.y);
+            four_halves(w ? vc[i].w : vc[i].y, x.z, x.w);
+            *reinterpret_cast<uint4*>(d0 + KV_BYTES + at) = x;
+          }
+        }
+      }
+      if (half) s_sv[st][key] = scale * down;
+      else s_sk[st][key] = scale;
+      uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0x55555555u;  // a bit every second lane
+      there = (there | there >> 1) & 0x33333333u;
+      there = (there | there >> 2) & 0x0f0f0f0fu;
+      there = (there | there >> 4) & 0x00ff00ffu;
+      there = (there | there >> 8) & 0x0000ffffu;
+      if (lane == 0) s_there[st][warp - CONVERT_WARP] = (uint16_t)there;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st]);
+      const int id = next_id;
+      if (j + 1 < n_tiles) {
+        fetch(j + 1, id);
+        next_id = page_of(j + 2);
+      }
+    }
+    if (!ok) failed = 1;
+    report_bad_page(bad, a.status);
+  } else if (warp >= MMA_WARP) {
+    // ---------------- MMA: a warp a unit
+    const int u = warp - MMA_WARP;
+    if (u < live_units) {
+      constexpr uint32_t idesc_qk = idesc_half(BQ, BKV);
+      constexpr uint32_t idesc_pv = idesc_half(BQ, HD) | (1u << 16);  // B operand MN-major
+      const uint32_t d_s = tmem + u * 256, d_o = d_s + 128;
+      const uint64_t q0 = make_desc(smem_u32(sQ + (streams ? 0 : u) * PIECES * Q_BYTES));
+      const uint64_t k0 = make_desc(smem_u32(ring)), v0 = make_desc_mn(smem_u32(ring + KV_BYTES));
+      const int first = streams ? u : 0;
+      const int n = (n_tiles - first + step - 1) / step;
+      bool ok = true;
+      auto issue_qk = [&](int j) {
+        const int t = first + j * step, st = t % STAGES;
+        if (!mbar_wait(&full[st], (t / STAGES) & 1)) return false;
+        tcgen05_fence_after();
+        __syncwarp();
+        const uint64_t kd = k0 + (uint64_t)(st * (2 * KV_BYTES / 16));
+#pragma unroll
+        for (int p = 0; p < PIECES; p++)
+#pragma unroll
+          for (int k = 0; k < HD / 16; k++)
+            umma_warp(d_s + (j & 1) * BKV, q0 + (uint64_t)(p * (Q_BYTES / 16) + (k >> 2) * (BQ * 128 / 16) + (k & 3) * 2),
+                      kd + (uint64_t)((k >> 2) * (BKV * 128 / 16) + (k & 3) * 2), idesc_qk, (p > 0 || k > 0) ? 1u : 0u);
+        commit_warp(&s_full[u][j & 1]);
+        return true;
+      };
+      ok = issue_qk(0);
+      for (int j = 0; j < n && ok; j++) {
+        if (j + 1 < n && !issue_qk(j + 1)) { ok = false; break; }
+        if (!mbar_wait(&p_full[u], j & 1)) { ok = false; break; }
+        tcgen05_fence_after();
+        __syncwarp();
+        const int t = first + j * step, st = t % STAGES;
+        const uint64_t vd = v0 + (uint64_t)(st * (2 * KV_BYTES / 16));
+#pragma unroll
+        for (int p = 0; p < PIECES; p++)
+#pragma unroll
+          for (int k = 0; k < BKV / 16; k++)
+            umma_a_tmem(d_o, d_s + (j & 1) * BKV + p * 32 + k * 8, vd + (uint64_t)(k * (2048 / 16)), idesc_pv, (j > 0 || p > 0 || k > 0) ? 1u : 0u);
+        commit_warp(&o_done[u]);
+        commit_warp(&empty[st]);
+      }
+      if (!ok) failed = 1;
+    }
+  } else if (unit < live_units) {
+    // ---------------- softmax and output: thread = row = lane of tensor memory
+    const int u = unit, first = streams ? u : 0;
+    const int n = (n_tiles - first + step - 1) / step;
+    if (streams) row_scale = unit_m[r];
+    const int pos = p0 + token;
+    const int low_pos = streams ? first_pos : p0 + (row0 + u * BQ) / a.group;  // of the unit's first and last row
+    const int high_pos = streams ? last_pos : p0 + (row0 + min((u + 1) * BQ, live_rows) - 1) / a.group;
+    const int lim_lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    const uint32_t span = (uint32_t)(pos - lim_lo);
+    const uint32_t s_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + u * 256, o_addr = s_addr + 128;
+    const uint64_t rs2 = twice(row_scale);
+    float m = NEG_BIG, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; j++) {
+      const int t = first + j * step, st = t % STAGES, key0 = k_begin + t * BKV;
+      if (!mbar_wait(&s_full[u][j & 1], (j >> 1) & 1)) { ok = false; break; }
+      tcgen05_fence_after();
+      uint32_t x[32], y[32];
+      tmem_ld32_issue(s_addr + (j & 1) * BKV, x);
+      tmem_ld32_issue(s_addr + (j & 1) * BKV + 32, y);
+      const uint2 there = *reinterpret_cast<const uint2*>(&s_there[st][0]);
+      const bool whole = (there.x & there.y) == 0xffffffffu && key0 + BKV - 1 <= low_pos && (a.window <= 0 || key0 > high_pos - a.window);
+      tmem_wait();
+      float top;
+      if (whole) {
+        top = max_nan(scale_max<false>(x, s_sk[st], 0, 0, 0), scale_max<false>(y, s_sk[st] + 32, 0, 0, 0));
+      } else {
+        top = max_nan(scale_max<true>(x, s_sk[st], lim_lo - key0, span, there.x), scale_max<true>(y, s_sk[st] + 32, lim_lo - key0 - 32, span, there.y));
+      }
+      top *= row_scale;
+      // (every tile's: a wait that leaves one out could take an older phase for the one it wants)
+      if (j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
+      const bool moves = !(top - m <= REF_SLACK);
+      if (__any_sync(0xffffffffu, moves)) {
+        // rows of this warp move their reference: O and l of those rows are scaled to the new one
+        const float m2 = moves ? max_nan(m, top) : m;
+        const float alpha = fast_exp2(m - m2);
+        if (j > 0) {
+          tcgen05_fence_after();
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16_issue(o_addr + c0, v);
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+            tmem_st16(o_addr + c0, v);
+          }
+        }
+        l *= alpha;
+        m = m2;
+      }
+      uint32_t hi[32], low[PIECES == 2 ? 32 : 1];
+      uint64_t sums = 0;
+      const uint64_t neg_m = twice(-m);
+      if (whole) {
+        weights<false, PIECES == 2>(x, s_sv[st], hi, low, rs2, neg_m, sums);
+        weights<false, PIECES == 2>(y, s_sv[st] + 32, hi + 16, low + (PIECES == 2 ? 16 : 0), rs2, neg_m, sums);
+      } else {
+        weights<true, PIECES == 2>(x, s_sv[st], hi, low, rs2, neg_m, sums);
+        weights<true, PIECES == 2>(y, s_sv[st] + 32, hi + 16, low + (PIECES == 2 ? 16 : 0), rs2, neg_m, sums);
+      }
+      tmem_st32(s_addr + (j & 1) * BKV, hi);
+      if constexpr (PIECES == 2) tmem_st32(s_addr + (j & 1) * BKV + 32, low);
+      uint32_t s0, s1;
+      split(sums, s0, s1);
+      l += __uint_as_float(s0) + __uint_as_float(s1);
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[u]);
+    }
+    if (ok && n > 0) ok = mbar_wait(&o_done[u], (n - 1) & 1);
+    tcgen05_fence_after();
+    // the units of one head's rows together: the second hands its output over through the ring (which both are through with
+    // when each has its last product)
+    float* other = reinterpret_cast<float*>(ring);
+    float other_w = 0.f, w = 1.f;
+    if (streams && live_units == 2) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 1) {
+        unit_m[r] = m;
+        unit_l[r] = l;
+        for (int c0 = 0; c0 < HD; c0 += 16) {
+          uint32_t v[16];
+          tmem_ld16_issue(o_addr + c0, v);
+          tmem_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i++) other[(c0 + i) * BQ + r] = __uint_as_float(v[i]);
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (u == 0) {
+        const float m2 = max_nan(m, unit_m[r]);
+        w = fast_exp2(m - m2);
+        other_w = fast_exp2(unit_m[r] - m2);
+        l = l * w + unit_l[r] * other_w;
+      }
+    }
+    if (ok && (!streams || u == 0)) {
+      const float factor = l == 0.f ? 0.f : __uint_as_float((unsigned)(127 - 10 + v_exp) << 23) / l;
+      T* dst = reinterpret_cast<T*>(a.out) + (a.q_start[s] + token) * a.out_stride + (long long)head * HD;
+      const bool wide = (((uintptr_t)dst) & 15) == 0;
+#pragma unroll 1
+      for (int c0 = 0; c0 < HD; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld16_issue(o_addr + c0, v);
+        tmem_wait();
+        float z[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          z[i] = __uint_as_float(v[i]) * w;
+          if (other_w != 0.f || other_w != other_w) z[i] = fmaf(other[(c0 + i) * BQ + r], other_w, z[i]);
+          z[i] *= factor;
+        }
+        if (!row_live) continue;
+        if (wide) {
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + c0 + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+              *reinterpret_cast<uint4*>(dst + c0 + i) =
+                  make_uint4(pack_bf16(z[i], z[i + 1]), pack_bf16(z[i + 2], z[i + 3]), pack_bf16(z[i + 4], z[i + 5]), pack_bf16(z[i + 6], z[i + 7]));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i++) dst[c0 + i] = from_float<T>(z[i]);
+        }
+      }
+    }
+    if (!ok) failed = 1;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+  if (tid == 0 && failed) atomicOr(a.status, TKB_STATUS_WAIT_TIMEOUT);
+}
+
+template <typename T>
+int launch(Args a, int portions, int tokens, cudaStream_t st) {
+  static SharedMemoryRequest ask;
+  int rc = ask({{(const void*)attn_kv8_tc_kernel<T>, Layout<T>::BYTES}});
+  if (rc) return rc;
+  auto items = [&](int rows) { return (long long)tokens * a.group / rows + portions; };
+  // (units that share their rows hold a tile each while they wait for the next: four stages)
+  a.rows = items(2 * BQ) * a.nkv >= sm_count() || Layout<T>::STAGES < 4 ? 2 * BQ : BQ;
+  const long long blocks = items(a.rows) * a.nkv;
+  if (blocks > 0x7fffffffll) return -3;
+  return launch_pdl(attn_kv8_tc_kernel<T>, dim3((unsigned)blocks), dim3(THREADS), (size_t)Layout<T>::BYTES, st, a);
+}
+
+}  // namespace
+
+// Requests that bring more than one token, `portions` of them with `tokens` tokens at most; the others are left out.
+TKB_EXPORT int tkb_attn_kv8_tc(const void* q, long long q_stride, void* out, long long out_stride, int f32, const void* kcache,
+                               const void* vcache, const float* k_scale, const float* v_scale, const int* q_start, const int* q_len,
+                               const int* kv_len, const int* page_indptr, const int* page_ids, int n_seqs, int portions, int tokens, int nh,
+                               int nkv, int ps, float scale, int window, int num_pages, int* status, void* st_) {
+  if (n_seqs <= 0 || portions <= 0 || tokens <= 0) return 0;
+  if (nkv <= 0 || nh <= 0 || nh % nkv || ps <= 0 || window < 0 || !(scale > 0.f)) return -2;
+  if ((long long)tokens * (nh / nkv) > 0x7fffff00ll) return -3;
+  Args a = {};
+  a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+  a.kcache = (const int8_t*)kcache, a.vcache = (const int8_t*)vcache, a.k_scale = k_scale, a.v_scale = v_scale;
+  a.q_start = q_start, a.q_len = q_len, a.kv_len = kv_len, a.page_indptr = page_indptr, a.page_ids = page_ids;
+  a.n_seqs = n_seqs, a.group = nh / nkv, a.nkv = nkv, a.ps = ps, a.window = window, a.num_pages = num_pages, a.status = status;
+  a.ps_shift = (ps & (ps - 1)) == 0 ? 31 - __builtin_clz(ps) : -1;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  return f32 ? launch<float>(a, portions, tokens, (cudaStream_t)st_) : launch<bf16>(a, portions, tokens, (cudaStream_t)st_);
+}

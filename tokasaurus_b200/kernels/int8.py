@@ -20,13 +20,15 @@ from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, 
 
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
 c_longlong = ctypes.c_longlong
+KV8_TC_MAX_DIM = 128  # head sizes whose scores and output fit tensor memory for two units
 
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _ARGS = {
     "tkb_quantise_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _P),
     "tkb_int8_product": (_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P),
-    "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _P, _P),
+    "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _I, _P, _P),
+    "tkb_attn_kv8_tc": (_P, _L, _P, _L, _I) + (_P,) * 9 + (_I,) * 6 + (_F, _I, _I, _P, _P),
     "tkb_attn_kv8_scratch": (_I,) * 6,
     "tkb_linear_int8": (_P, _L, _I, _P, _L, _P, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P),
 }
@@ -220,7 +222,7 @@ def read_kv8(kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, 
 def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
              q_start: torch.Tensor, q_len: torch.Tensor, kv_len: torch.Tensor, page_indptr: torch.Tensor, page_ids: torch.Tensor,
              n_heads: int, n_kv_heads: int, head_dim: int, page_size: int, scale: float, window: int | None, status: torch.Tensor,
-             max_q_len: int, max_kv_len: int, single_tokens: int) -> None:
+             max_q_len: int, max_kv_len: int, single_tokens: int, portions: int | None = None) -> None:
     """Causal grouped-query attention of a step's tokens over a cache held in 8 bits.
 
     q: rotated queries, the first n_heads*head_dim columns of rows [T, >= that] (bfloat16 or float32); out: [T, n_heads*head_dim]
@@ -228,8 +230,9 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     (``page_ids`` from ``page_indptr[s]`` on) hold; the tokens must have been written before.  A token sees the keys up to its own
     position, with ``window`` only the last so many, none on pages given back (id -1); one that sees none gets 0.
 
-    Bounds known to the host, from which the launch is sized: ``max_q_len`` and ``max_kv_len`` over all requests,
-    ``single_tokens``: how many requests bring one token (requests beyond these bounds are not computed whole)."""
+    What the host knows, from which launches are made and sized: ``max_q_len`` and ``max_kv_len`` over all requests;
+    ``single_tokens``, how many requests bring one token; ``portions``, how many bring more (by default all the others).  For a
+    launch that is replayed with other requests each is the most there will be (requests that bring none count nowhere)."""
     what = "attn_kv8"
     _need_cuda(q, out, kcache, vcache, k_scale, v_scale, q_start, q_len, kv_len, page_indptr, page_ids, status)
     f32 = _is_f32(q.dtype)
@@ -244,16 +247,31 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     n = q_len.numel()
     _need(q_start.numel() >= n and kv_len.numel() >= n and page_indptr.numel() > n, f"{what}: a start, a length and pages for every request")
     _need(window is None or window >= 1, f"{what}: a window of one key at least")
-    _need(max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n, f"{what}: bounds")
+    _need(scale > 0, f"{what}: scores are scaled by a positive number")
+    _need(max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n and (portions is None or portions >= 0), f"{what}: bounds")
     T = q.shape[0]
     if n == 0 or T == 0:
         return
     group = n_heads // n_kv_heads
     singles = min(single_tokens, T)
-    scratch = torch.empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(n, singles, T, max_kv_len, n_kv_heads, group),),
+    exact = portions is None
+    portions = (n - singles if exact else min(portions, n)) if max_q_len > 1 else 0
+    which, tokens, requests = 3, T, n
+    if head_dim <= KV8_TC_MAX_DIM:
+        # portions on the tcgen05 tensor cores, single tokens with their keys cut over the GPU
+        if portions:
+            _check(_entry("attention_kv8_tc.cu", "tkb_attn_kv8_tc", head_dim)(
+                q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
+                n, portions, T - singles if exact else T, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0],
+                status.data_ptr(), _stream()), what)
+        if singles == 0:
+            return
+        which, tokens, requests = 1, singles, singles
+    scratch = torch.empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group),),
                           dtype=torch.uint8, device=q.device)
     _check(_entry("attention_kv8.cu", "tkb_attn_kv8", head_dim)(
         q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
         v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
-        scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0],
+        scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0], which,
         status.data_ptr(), _stream()), what)

@@ -49,7 +49,8 @@ def family_modules() -> list[tuple[str, dict | None]]:
 
 def int8_modules(head_dims=()) -> list[tuple[str, dict | None]]:
     """Products in 8-bit integers, and the cache held in 8 bits with the attention over it."""
-    return [("int8_product.cu", None), ("cache8.cu", None)] + [("attention_kv8.cu", {"TKB_HD": hd}) for hd in head_dims]
+    return [("int8_product.cu", None), ("cache8.cu", None)] + [
+        (source, {"TKB_HD": hd}) for hd in head_dims for source in ("attention_kv8.cu", "attention_kv8_tc.cu") if hd <= 128 or source == "attention_kv8.cu"]
 
 
 def optional_modules(head_dim: int) -> list[tuple[str, dict | None]]:
