@@ -541,7 +541,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int key_row = key_of_row(g);  // this lane's key rows of a group: key_row, key_row + 8
     constexpr int MINE = COLS / WARPS;  // columns whose queries (and results) a warp brings in (out)
     constexpr int N4 = (HD / 4 + 31) / 32;  // four numbers (a word of codes) of a query a lane and turn
-    float raw[MINE][N4][4];
+    T raw[MINE][N4][4];
     auto load_queries = [&](const Walk& x) {
 #pragma unroll
       for (int y = 0; y < MINE; y++) {
@@ -554,9 +554,13 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const int d = (lane + 32 * i) * 4 + e;
-            raw[y][i][e] = real && d < HD ? to_float(src[d]) : 0.f;
+            raw[y][i][e] = src[HD % 128 == 0 ? d : min(d, HD - 1)];  // (no branch: the loads are to be on their way together)
           }
       }
+    };
+    auto number = [&](const Walk& x, int y, int i, int e) {
+      const bool real = x.ct * COLS + warp + WARPS * y < x.r.q_len * a.out.group && (lane + 32 * i) * 4 < HD;
+      return real ? to_float(raw[y][i][e]) : 0.f;
     };
     if (more(w)) load_queries(w);
     auto holds_whole = [](const Walk& x) { return x.tile == 0 && x.tile_end == x.r.tiles; };
@@ -569,10 +573,14 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       for (int y = 0; y < MINE; y++) {
         const int j = warp + WARPS * y;
         unsigned top = 0;
+        float v[N4][4];
 #pragma unroll
         for (int i = 0; i < N4; i++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(raw[y][i][e]) & 0x7fffffffu);
+          for (int e = 0; e < 4; e++) {
+            v[i][e] = number(w, y, i, e);
+            top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+          }
         top = __reduce_max_sync(0xffffffffu, top);
         // by a power of two to [1, 2) (what is below 2^-126 stays there), then to the fixed point's unit
         const int e = max(1, (int)(top >> 23)) - 127;
@@ -589,7 +597,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
             uint32_t piece[QP] = {};
 #pragma unroll
             for (int b = 0; b < 4; b++) {
-              int x = some ? __float2int_rn(raw[y][i][b] * down * f) : 0;
+              int x = some ? __float2int_rn(v[i][b] * down * f) : 0;
 #pragma unroll
               for (int p = QP - 1; p >= 0; p--) {
                 const int low = p == 0 ? x : (int)(int8_t)(x & 0xff);

@@ -9,94 +9,240 @@
 // each step rounded once in float32.  A page's first slot always starts it afresh: what an earlier request left there does
 // not count.  An infinity or NaN among the numbers makes the block's scale NaN: all that is read from the block is NaN then.
 // Writing the same tokens again changes nothing (their scale has been reached).
-#include "common.cuh"
+#include "int8.cuh"
+
+#include <type_traits>
 
 using namespace tkb;
 
 namespace {
 
-constexpr float ONE_127TH = 1.f / 127.f;
+// A block takes a kv head and a window of `per` tokens and writes the segments that lead in it: four warps a side, each every fourth
+// row of a chunk of 16.  A warp's numbers of a chunk are asked for together and stay in registers between the search for the
+// largest and the codes (segments of several chunks are read twice).  A block for every token behind these rotates its q heads.
+// What bounds it: the latency of the lookups and of the rows in small steps, the rows' bytes in long ones.  (A warp a head and
+// side with all 16 rows: 8,000 prompt tokens of 8 kv heads of 128 37 us.)
+constexpr int SIDE_WARPS = 4, W_THREADS = 2 * SIDE_WARPS * 32, CHUNK = 16;
 
-__device__ __forceinline__ int code_of(float x, float s) {
-  return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f);
+// Four numbers as they lie in memory, and as float32: apart, so that many loads can be on their way.
+__device__ __forceinline__ float4 raw_four(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ uint2 raw_four(const __nv_bfloat16* p) { return *reinterpret_cast<const uint2*>(p); }
+__device__ __forceinline__ float4 four_of(float4 v) { return v; }
+__device__ __forceinline__ float4 four_of(uint2 v) {
+  return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
-
-// Element d of a head after the rotation (half-split pairs), at angles pos * inv_freq.
-template <typename T>
-__device__ __forceinline__ float rotated(const T* x, int d, int half, int rot, float pos, const float* __restrict__ inv_freq) {
-  if (d >= rot) return to_float(x[d]);
-  const int j = d < half ? d : d - half;
-  float sn, c;
-  sincosf(pos * inv_freq[j], &sn, &c);
-  return d < half ? to_float(x[d]) * c - to_float(x[d + half]) * sn : to_float(x[d]) * c + to_float(x[j]) * sn;
+template <typename T> __device__ __forceinline__ float4 load_four(const T* p) { return four_of(raw_four(p)); }
+template <typename T> __device__ __forceinline__ void store_four(T* p, float4 v);
+template <> __device__ __forceinline__ void store_four(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+template <> __device__ __forceinline__ void store_four(__nv_bfloat16* p, float4 v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
-
-constexpr int W_THREADS = 256;
-
+// Numbers d .. d + 3 (v) of a head after the rotation (half-split pairs; half a multiple of 4): y their partners, cs the token's
+// cosines, then its sines.
+__device__ __forceinline__ float4 rotated_four(float4 v, float4 y, int d, int half, const float* cs) {
+  if (d >= 2 * half) return v;
+  const bool low = d < half;
+  const int j = low ? d : d - half;
+  const float4 c = *reinterpret_cast<const float4*>(cs + j), sn = *reinterpret_cast<const float4*>(cs + half + j);
+  if (low) return make_float4(v.x * c.x - y.x * sn.x, v.y * c.y - y.y * sn.y, v.z * c.z - y.z * sn.z, v.w * c.w - y.w * sn.w);
+  return make_float4(v.x * c.x + y.x * sn.x, v.y * c.y + y.y * sn.y, v.z * c.z + y.z * sn.z, v.w * c.w + y.w * sn.w);
+}
+// The same number by number, for other halves.
 template <typename T>
-__global__ void __launch_bounds__(W_THREADS)
+__device__ __forceinline__ float4 rotated_each(const T* x, int d, int half, const float* cs) {
+  float r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int k = d + e;
+    r[e] = to_float(x[k]);
+    if (k < half) r[e] = r[e] * cs[k] - to_float(x[k + half]) * cs[half + k];
+    else if (k < 2 * half) r[e] = r[e] * cs[k - half] + to_float(x[k - half]) * cs[k];
+  }
+  return make_float4(r[0], r[1], r[2], r[3]);
+}
+template <typename T, int WORDS, bool ROT>
+__global__ void __launch_bounds__(W_THREADS, WORDS > 4 ? 2 : ROT ? 4 : 5)
 rope_kv8_write_kernel(T* __restrict__ qkv, const int* __restrict__ positions, const int* __restrict__ token_seq,
                       const int* __restrict__ page_indptr, const int* __restrict__ page_ids, const float* __restrict__ inv_freq,
                       int8_t* __restrict__ kcache, int8_t* __restrict__ vcache, float* __restrict__ k_scale,
-                      float* __restrict__ v_scale, int T_, int nh, int nkv, int hd, int rot, int ps, int num_pages, int write_cache,
-                      int* __restrict__ status) {
+                      float* __restrict__ v_scale, int tokens, int per, int nh, int nkv, int hd, int rot, unsigned word_mul, int ps,
+                      int ps_shift, int num_pages, int writers, int* __restrict__ status) {
+  extern __shared__ __align__(16) float cs[];  // [CHUNK][rot]
+  __shared__ unsigned s_top[2 * SIDE_WARPS];
   trigger_dependents();
-  const int t = blockIdx.x;
-  const int s = token_seq[t];
-  if (s < 0) return;  // padding
-  const int pos = positions[t];
-  const int half = rot >> 1;
-  const long long C = (long long)(nh + 2 * nkv) * hd;
   grid_dependency_wait();
-  T* row = qkv + t * C;
-  for (int i = threadIdx.x; i < nh * half; i += W_THREADS) {
-    const int h = i / half, j = i - h * half;
-    T* p = row + h * hd + j;
-    const float a = to_float(p[0]), b = to_float(p[half]);
-    float sn, c;
-    sincosf((float)pos * inv_freq[j], &sn, &c);
-    p[0] = from_float<T>(a * c - b * sn);
-    p[half] = from_float<T>(b * c + a * sn);
-  }
-  if (!write_cache) return;
-  const int slot = pos % ps;
-  if (slot != 0 && t > 0 && token_seq[t - 1] == s) return;  // an earlier token leads this one's segment
-  int n = 1;
-  while (slot + n < ps && t + n < T_ && token_seq[t + n] == s) n++;
-  const int page = page_ids[page_indptr[s] + pos / ps];
-  if (page < 0 || page >= num_pages) {
-    if (threadIdx.x == 0) atomicOr(status, TKB_STATUS_BAD_PAGE);
-    return;
-  }
-  const int lane = threadIdx.x & 31;
-  for (int task = threadIdx.x >> 5; task < 2 * nkv; task += W_THREADS / 32) {
-    const int h = task >> 1;
-    const bool is_v = task & 1;
-    const T* src = row + (long long)(nh + (is_v ? nkv : 0) + h) * hd;
-    const int r = is_v ? 0 : rot;
-    int8_t* dst = (is_v ? vcache : kcache) + ((long long)page * nkv + h) * ps * hd;
-    float* scale = (is_v ? v_scale : k_scale) + (long long)page * nkv + h;
-    unsigned top = 0;
-    for (int i = 0; i < n; i++)
-      for (int d = lane; d < hd; d += 32)
-        top = max(top, __float_as_uint(rotated(src + i * C, d, r >> 1, r, (float)(pos + i), inv_freq)) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    const float old = slot == 0 ? 0.f : *scale;
-    float s2 = top < 0x7f800000u ? __uint_as_float(top) * ONE_127TH : NAN;
-    if (!(s2 > old)) s2 = (s2 == s2) ? old : s2;  // (a NaN stays one, whichever side it is on)
-    const bool some = s2 > 0.f;
-    if (s2 != old) {
-      for (int i = lane; i < ps * hd; i += 32) {
-        const int sl = i / hd;
-        if (sl < slot || sl >= slot + n) dst[i] = some ? (int8_t)code_of((float)dst[i] * old, s2) : (int8_t)0;
+  const int half = rot >> 1, words = hd >> 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long C = (long long)(nh + 2 * nkv) * hd;
+  auto angles = [&](int pos, int n) {  // of n rows from position pos on
+    for (int i = threadIdx.x; i < n * half; i += W_THREADS) {
+      const int r = i / half, j = i - r * half;
+      float sn, c;
+      sincosf((float)(pos + r) * inv_freq[j], &sn, &c);
+      cs[r * rot + j] = c;
+      cs[r * rot + half + j] = sn;
+    }
+  };
+  if (ROT && (int)blockIdx.x >= writers) {
+    // ---------------- a token's q heads
+    const int t = blockIdx.x - writers;
+    if (token_seq[t] < 0) return;
+    angles(positions[t], 1);
+    __syncthreads();
+    T* row = qkv + t * C;
+    if ((half & 3) == 0) {
+      for (int i = threadIdx.x; i < nh * (half >> 2); i += W_THREADS) {
+        const int h = i / (half >> 2), j = (i - h * (half >> 2)) * 4;
+        T* p = row + (long long)h * hd + j;
+        const float4 a = load_four(p), b = load_four(p + half);
+        const float4 c = *reinterpret_cast<const float4*>(cs + j), sn = *reinterpret_cast<const float4*>(cs + half + j);
+        store_four(p, make_float4(a.x * c.x - b.x * sn.x, a.y * c.y - b.y * sn.y, a.z * c.z - b.z * sn.z, a.w * c.w - b.w * sn.w));
+        store_four(p + half, make_float4(b.x * c.x + a.x * sn.x, b.y * c.y + a.y * sn.y, b.z * c.z + a.z * sn.z, b.w * c.w + a.w * sn.w));
+      }
+    } else {
+      for (int i = threadIdx.x; i < nh * half; i += W_THREADS) {
+        const int h = i / half, j = i - h * half;
+        T* p = row + (long long)h * hd + j;
+        const float a = to_float(p[0]), b = to_float(p[half]);
+        p[0] = from_float<T>(a * cs[j] - b * cs[half + j]);
+        p[half] = from_float<T>(b * cs[j] + a * cs[half + j]);
       }
     }
-    for (int i = 0; i < n; i++)
-      for (int d = lane; d < hd; d += 32) {
-        const float x = rotated(src + i * C, d, r >> 1, r, (float)(pos + i), inv_freq);
-        dst[(slot + i) * hd + d] = some ? (int8_t)code_of(x, s2) : (int8_t)0;
+    return;
+  }
+  // ---------------- the segments that lead in this block's window of tokens: a lane looks at a token
+  const int kvh = blockIdx.x % nkv, t0 = blockIdx.x / nkv * per, mine = t0 + lane;
+  int my_s = -1, my_pos = 0, my_slot = 0, my_page = -1;
+  bool leads = false, ends = true;  // ends: what stands ahead of the token is over
+  if (lane < per && mine < tokens) {
+    my_s = token_seq[mine];
+    const int before = mine > 0 ? token_seq[mine - 1] : -1;
+    my_pos = positions[mine];
+    const int in_table = ps_shift >= 0 ? my_pos >> ps_shift : my_pos / ps;
+    my_slot = my_pos - in_table * ps;
+    leads = my_s >= 0 && (my_slot == 0 || before != my_s);
+    ends = leads || my_s < 0;
+    if (leads) my_page = page_ids[page_indptr[my_s] + in_table];
+  }
+  const bool is_v = warp >= SIDE_WARPS;
+  const int part = warp % SIDE_WARPS, side_thread = threadIdx.x % (SIDE_WARPS * 32), my_half = is_v ? 0 : half;
+  int8_t* const cache = is_v ? vcache : kcache;
+  float* const scales = is_v ? v_scale : k_scale;
+  const unsigned boundary = __ballot_sync(0xffffffffu, ends);
+  bool first = true;
+  for (unsigned todo = __ballot_sync(0xffffffffu, leads); todo != 0; todo &= todo - 1) {
+    const int at = __ffs(todo) - 1;
+    const int s = __shfl_sync(0xffffffffu, my_s, at), pos = __shfl_sync(0xffffffffu, my_pos, at), slot = __shfl_sync(0xffffffffu, my_slot, at);
+    const int page = __shfl_sync(0xffffffffu, my_page, at), t = t0 + at;
+    if (page < 0 || page >= num_pages) {
+      if (threadIdx.x == 0) atomicOr(status, TKB_STATUS_BAD_PAGE);
+      continue;
+    }
+    const long long block = (long long)page * nkv + kvh;
+    const float old = slot != 0 ? scales[block] : 0.f;
+    // tokens of the segment: to the next boundary; from the window's end on (every lane from `per` on is one) as far as they follow
+    const unsigned later = at == 31 ? 0u : boundary & (~0u << (at + 1));
+    int n = (later ? __ffs(later) - 1 : 32) - at;
+    const int most = min(ps - slot, tokens - t);
+    if (at + n >= per) {
+      while (n < most) {
+        const unsigned same = __ballot_sync(0xffffffffu, n + lane < most && token_seq[t + n + lane] == s);
+        const int k = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+        n += k;
+        if (k < 32) break;
       }
-    if (lane == 0) *scale = s2;
+    }
+    const bool one = n <= CHUNK;
+    const T* const rows = qkv + t * C + (long long)(nh + (is_v ? nkv : 0) + kvh) * hd;
+    if (!first) __syncthreads();  // (the segment before is through with the angles and the largest)
+    first = false;
+    // A warp's words (four numbers each) of a chunk of m rows from c0 on: word i of its rows together is lane i % 32's.  All are asked
+    // for before the first is used and without a branch (lanes beyond the last word ask for that one).
+    float4 x[WORDS];
+    auto load = [&](int c0, int m) {
+      const int count = ((m - part + SIDE_WARPS - 1) / SIDE_WARPS) * words, last = max(count - 1, 0);
+      auto place = [&](int u, int& r, int& d) {
+        const int k = min(lane + 32 * u, last);
+        r = (int)__umulhi((unsigned)k, word_mul);
+        d = 4 * (k - r * words);
+        r = min(r * SIDE_WARPS + part, m - 1);
+      };
+      if (ROT && (half & 3) != 0) {
+#pragma unroll
+        for (int u = 0; u < WORDS; u++) {
+          int r, d;
+          place(u, r, d);
+          x[u] = rotated_each(rows + (c0 + r) * C, d, my_half, cs + r * rot);
+        }
+      } else {
+        decltype(raw_four(rows)) a[WORDS], b[ROT ? WORDS : 1];
+#pragma unroll
+        for (int u = 0; u < WORDS; u++) {
+          int r, d;
+          place(u, r, d);
+          const T* row = rows + (c0 + r) * C;
+          a[u] = raw_four(row + d);
+          if constexpr (ROT) b[u] = raw_four(row + (d < my_half ? d + my_half : d < 2 * my_half ? d - my_half : d));
+        }
+#pragma unroll
+        for (int u = 0; u < WORDS; u++) {
+          int r, d;
+          place(u, r, d);
+          x[u] = four_of(a[u]);
+          if constexpr (ROT) x[u] = rotated_four(x[u], four_of(b[u]), d, my_half, cs + r * rot);
+        }
+      }
+    };
+    auto bring_angles = [&](int c0, int m) {
+      if (!ROT) return;
+      if (c0 > 0 || !one) __syncthreads();
+      angles(pos + c0, m);
+      __syncthreads();
+    };
+    unsigned top = 0;
+    for (int c0 = 0; c0 < n; c0 += CHUNK) {
+      const int m = min(CHUNK, n - c0);
+      bring_angles(c0, m);
+      load(c0, m);
+      if (part < m) {
+#pragma unroll
+        for (int u = 0; u < WORDS; u++) top = max(max(top, max(magnitude(x[u].x), magnitude(x[u].y))), max(magnitude(x[u].z), magnitude(x[u].w)));
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SIDE_WARPS; i++) top = max(top, s_top[(is_v ? SIDE_WARPS : 0) + i]);
+    float sc = top < NOT_FINITE ? __uint_as_float(top) * ONE_127TH : NAN;
+    if (!(sc > old)) sc = sc == sc ? old : sc;  // (a NaN stays one, whichever side it is on)
+    const bool some = sc > 0.f;
+    const float inv = 1.f / sc;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(cache) + block * ps * words;
+    for (int c0 = 0; c0 < n; c0 += CHUNK) {
+      const int m = min(CHUNK, n - c0), count = ((m - part + SIDE_WARPS - 1) / SIDE_WARPS) * words;
+      if (!one) {
+        bring_angles(c0, m);
+        load(c0, m);
+      }
+#pragma unroll
+      for (int u = 0; u < WORDS; u++) {
+        const int i = lane + 32 * u, r = (int)__umulhi((unsigned)i, word_mul);
+        if (part < m && i < count) dst[(slot + c0 + r * SIDE_WARPS + part) * words + i - r * words] = some ? four_codes(x[u], sc, inv) : 0u;
+      }
+    }
+    if (slot == 0 || sc != old) {
+      // the block's other codes, brought to the new scale
+      const int from = slot * words, kept = ps * words - n * words;
+#pragma unroll 2
+      for (int i = side_thread; i < kept; i += SIDE_WARPS * 32) {
+        const int k = i < from ? i : i + n * words;
+        const uint32_t c = old == 0.f ? 0u : dst[k];
+        const float4 v = make_float4((float)(int8_t)c * old, (float)(int8_t)(c >> 8) * old, (float)(int8_t)(c >> 16) * old, (float)(int8_t)(c >> 24) * old);
+        dst[k] = some ? four_codes(v, sc, inv) : 0u;
+      }
+      if (side_thread == 0) scales[block] = sc;
+    }
   }
 }
 
@@ -129,14 +275,30 @@ TKB_EXPORT int tkb_rope_kv8_write(void* qkv, int f32, const int* positions, cons
                                   int tokens, int nh, int nkv, int hd, int rot, int ps, int num_pages, int write_cache, int* status, void* st_) {
   if (tokens <= 0) return 0;
   if (rot < 0 || rot > hd || (rot & 1) || (hd & 15) || nh <= 0 || nkv <= 0 || ps <= 0) return -2;
-  cudaStream_t st = (cudaStream_t)st_;
-  if (f32)
-    return launch_pdl(rope_kv8_write_kernel<float>, dim3(tokens), dim3(W_THREADS), 0, st, (float*)qkv, positions, token_seq, page_indptr,
-                      page_ids, inv_freq, (int8_t*)kcache, (int8_t*)vcache, k_scale, v_scale, tokens, nh, nkv, hd, rot, ps, num_pages,
-                      write_cache, status);
-  return launch_pdl(rope_kv8_write_kernel<__nv_bfloat16>, dim3(tokens), dim3(W_THREADS), 0, st, (__nv_bfloat16*)qkv, positions, token_seq,
-                    page_indptr, page_ids, inv_freq, (int8_t*)kcache, (int8_t*)vcache, k_scale, v_scale, tokens, nh, nkv, hd, rot, ps,
-                    num_pages, write_cache, status);
+  if (hd > 256) return -2;
+  // windows that leave about 256 writers a head: of one token in steps of few, of a page of 16 in long ones
+  const int per = tokens <= 256 ? 1 : tokens >= 4096 ? 16 : (tokens + 255) / 256;
+  const long long writers = write_cache ? (long long)((tokens + per - 1) / per) * nkv : 0, blocks = writers + (rot ? tokens : 0);
+  if (blocks > 0x7fffffffll) return -3;
+  if (blocks == 0) return 0;
+  const int ps_shift = (ps & (ps - 1)) == 0 ? 31 - __builtin_clz(ps) : -1;
+  const size_t smem = (size_t)CHUNK * rot * 4;
+  const unsigned word_mul = hd > 4 ? 0xffffffffu / (unsigned)(hd / 4) + 1u : 0u;
+  auto go = [&](auto* rows, auto most, auto turns) {
+    using T = std::remove_pointer_t<decltype(rows)>;
+    constexpr auto kernel = rope_kv8_write_kernel<T, decltype(most)::value, decltype(turns)::value>;
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(W_THREADS), smem, (cudaStream_t)st_, rows, positions, token_seq, page_indptr,
+                      page_ids, inv_freq, (int8_t*)kcache, (int8_t*)vcache, k_scale, v_scale, tokens, per, nh, nkv, hd, rot, word_mul, ps, ps_shift,
+                      num_pages, (int)writers, status);
+  };
+  auto by_type = [&](auto most) {
+    if (rot == 0) return f32 ? go((float*)qkv, most, std::false_type()) : go((__nv_bfloat16*)qkv, most, std::false_type());
+    return f32 ? go((float*)qkv, most, std::true_type()) : go((__nv_bfloat16*)qkv, most, std::true_type());
+  };
+  // words of four rows that a lane has
+  if (hd <= 64) return by_type(std::integral_constant<int, 2>());
+  if (hd <= 128) return by_type(std::integral_constant<int, 4>());
+  return by_type(std::integral_constant<int, 8>());
 }
 
 // k_out, v_out: float32 [n, nkv, block]; block = page size * head size (a multiple of 16).

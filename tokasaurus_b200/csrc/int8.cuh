@@ -1,0 +1,38 @@
+// Numbers held in 8 bits: a code in [-127, 127] times a float32 scale, scale = max|x| * (1 / 127), code = rint(x / scale).
+#pragma once
+#include "common.cuh"
+
+namespace tkb {
+
+constexpr float ONE_127TH = 1.f / 127.f;
+
+// rint(x / s) with the quotient rounded as float32 division rounds it, held to [-127, 127].  A call: a division in place for every
+// number of an unrolled loop is what such a kernel then waits for, as instructions.
+__device__ __noinline__ int divided_code(float x, float s) { return (int)fminf(fmaxf(rintf(__fdiv_rn(x, s)), -127.f), 127.f); }
+
+// The codes of four numbers under scale s (> 0) as the bytes of a word; inv: 1 / s.  x * inv is within 3e-5 of the quotient, which
+// settles all but those next to a half (2 in 10,000) and those of a scale whose reciprocal is infinite: they are divided.  Adding
+// 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits (rintf and a conversion to int take the
+// unit that has a quarter of the rate).
+__device__ __forceinline__ uint32_t four_codes(const float4 x, float s, float inv) {
+  constexpr float ROUND = 12582912.f;
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  uint32_t b[4];
+  bool near = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float t = v[i] * inv, r = t + ROUND;
+    b[i] = __float_as_uint(r);
+    near |= !(fabsf(t - (r - ROUND)) <= 0.4999f);  // (or no number, of an infinite reciprocal)
+  }
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = (uint32_t)divided_code(v[i], s);
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+// Magnitudes as integers: NaN > infinity > every number.
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+constexpr unsigned NOT_FINITE = 0x7f800000u;  // magnitudes from here on
+
+}  // namespace tkb

@@ -11,22 +11,12 @@
 // memory), fed by TMA in boxes of 128 codes (one 128-byte swizzle row) a row.  Every wait on an mbarrier is bounded: after
 // the limit the block sets TKB_STATUS_WAIT_TIMEOUT, stops waiting, frees its tensor memory and returns.
 #include "tcgen05.cuh"
+#include "int8.cuh"
 #include "per_device.h"
 
 using namespace tkb5;
 
 namespace {
-
-constexpr float ONE_127TH = 1.f / 127.f;
-
-// rint(x / s) with the quotient rounded as float32 division rounds it, held to [-127, 127].  x * (1 / s) is within 3e-5 of
-// it, which settles all but quotients next to a half: those (2 in 10,000) are divided.
-__device__ __forceinline__ int code_of(float x, float s, float inv) {
-  const float t = x * inv;
-  float q = rintf(t);
-  if (!(fabsf(t - q) <= 0.4999f)) q = rintf(__fdiv_rn(x, s));
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
-}
 
 // A block a row.  A thread's numbers (up to CHUNKS times eight, as they were loaded) stay in registers between the search for
 // the largest and the codes; what a row has beyond that is read again.  WIDE: rows start on 16-byte boundaries and are
@@ -72,9 +62,8 @@ quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
   const int eights = K >> 3, step = blockDim.x;
   const int tail = (eights << 3) + threadIdx.x;  // the last K % 8 numbers: the first threads' own
   Eight<T, WIDE> mine[CHUNKS];
-  // magnitudes as integers: NaN > infinity > every number
   unsigned top = 0;
-  auto see = [&](float v) { top = max(top, __float_as_uint(v) & 0x7fffffffu); };
+  auto see = [&](float v) { top = max(top, magnitude(v)); };
 #pragma unroll
   for (int c = 0; c < CHUNKS; c++) {
     const int e = threadIdx.x + c * step;
@@ -99,17 +88,15 @@ quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
   __syncthreads();
   const int lane = threadIdx.x & 31;
   top = __reduce_max_sync(0xffffffffu, lane < (step >> 5) ? s_top[lane] : 0u);
-  const bool finite = top < 0x7f800000u;
+  const bool finite = top < NOT_FINITE;
   const float s = finite ? __uint_as_float(top) * ONE_127TH : NAN;
   const float inv = 1.f / s;
   const bool some = finite && s > 0.f;
   auto put = [&](int e, const Eight<T, WIDE>& v) {
-    uint32_t w[2] = {0, 0};
-    if (some) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)(uint8_t)code_of(v.at(i), s, inv) << (8 * (i & 3));
-    }
-    *reinterpret_cast<uint2*>(dst + 8 * e) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(dst + 8 * e) =
+        some ? make_uint2(four_codes(make_float4(v.at(0), v.at(1), v.at(2), v.at(3)), s, inv),
+                          four_codes(make_float4(v.at(4), v.at(5), v.at(6), v.at(7)), s, inv))
+             : make_uint2(0, 0);
   };
 #pragma unroll
   for (int c = 0; c < CHUNKS; c++) {
@@ -121,7 +108,7 @@ quantise_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
     v.load(row + 8 * e);
     put(e, v);
   }
-  if (tail < K) dst[tail] = some ? (int8_t)code_of(last, s, inv) : (int8_t)0;
+  if (tail < K) dst[tail] = some ? (int8_t)divided_code(last, s) : (int8_t)0;
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
 

@@ -11,15 +11,13 @@ NaN, and all that is computed from it is NaN.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int
 
 import torch
 
 from tokasaurus_b200.kernels import ops
-from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, _need_cuda, _ptr, _stream, _suffix, check_head_dim
+from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, _need_cuda, _stream, _suffix, check_head_dim
 
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
-c_longlong = ctypes.c_longlong
 KV8_TC_MAX_DIM = 128  # head sizes whose scores and output fit tensor memory for two units
 
 
@@ -27,6 +25,8 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_floa
 _ARGS = {
     "tkb_quantise_rows": (_P, _L, _I, _P, _L, _P, _I, _I, _P),
     "tkb_int8_product": (_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P),
+    "tkb_rope_kv8_write": (_P, _I) + (_P,) * 9 + (_I,) * 8 + (_P, _P),
+    "tkb_read_kv8": (_P,) * 7 + (_I,) * 4 + (_P, _P),
     "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _I, _P, _P),
     "tkb_attn_kv8_tc": (_P, _L, _P, _L, _I) + (_P,) * 9 + (_I,) * 6 + (_F, _I, _I, _P, _P),
     "tkb_attn_kv8_scratch": (_I,) * 6,
@@ -155,18 +155,23 @@ def lay_out_codes(w: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------------------------
-def _check_cache(what: str, kcache, vcache, k_scale, v_scale, n_kv_heads: int, page_size: int, head_dim: int) -> None:
-    for c, s in ((kcache, k_scale), (vcache, v_scale)):
-        _need(c.dtype == torch.int8 and c.is_contiguous() and c.dim() == 4 and tuple(c.shape[1:]) == (n_kv_heads, page_size, head_dim),
-              f"{what}: the cache is int8 [pages, kv heads, page size, head size]")
-        _need(s.dtype == torch.float32 and s.is_contiguous() and tuple(s.shape) == tuple(c.shape[:2]), f"{what}: scales are float32 [pages, kv heads]")
-        _need(c.data_ptr() % 16 == 0, f"{what}: the cache starts on a 16-byte boundary")
-    _need(kcache.shape[0] == vcache.shape[0], f"{what}: as many pages of keys as of values")
+def _check_cache(what: str, kcache, vcache, k_scale, v_scale, n_kv_heads: int, page_size: int, head_dim: int) -> int:
+    """The number of pages."""
+    shape = kcache.shape
+    if not (len(shape) == 4 and kcache.dtype == vcache.dtype == torch.int8 and shape == vcache.shape and shape[1] == n_kv_heads
+            and shape[2] == page_size and shape[3] == head_dim and kcache.is_contiguous() and vcache.is_contiguous()
+            and kcache.data_ptr() % 16 == 0 and vcache.data_ptr() % 16 == 0):
+        raise KernelError(f"{what}: keys and values are int8 [pages, kv heads, page size, head size] each, contiguous, on a 16-byte boundary")
+    if not (k_scale.dtype == v_scale.dtype == torch.float32 and k_scale.shape == v_scale.shape == shape[:2] and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise KernelError(f"{what}: scales are float32 [pages, kv heads], contiguous")
+    return shape[0]
 
 
-def _need_i32(what: str, **tensors) -> None:
-    for name, t in tensors.items():
-        _need(t.dtype == torch.int32 and t.is_contiguous(), f"{what}: {name} is int32, contiguous")
+def _check_i32(what: str, *tensors) -> None:
+    for t in tensors:
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: positions, request rows, lengths and page tables are int32, contiguous")
 
 
 def rope_kv8_write(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, page_indptr: torch.Tensor,
@@ -183,39 +188,44 @@ def rope_kv8_write(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.
     what = "rope_kv8_write"
     _need_cuda(qkv, positions, token_seq, page_indptr, page_ids, inv_freq, kcache, vcache, k_scale, v_scale, status)
     f32 = _is_f32(qkv.dtype)
-    n = qkv.shape[0]
-    _need(n_heads >= 1 and n_kv_heads >= 1 and page_size >= 1, f"{what}: sizes")
+    if n_heads < 1 or n_kv_heads < 1 or page_size < 1:
+        raise KernelError(f"{what}: sizes")
     check_head_dim(head_dim)
-    _need(qkv.dim() == 2 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim, f"{what}: qkv shape")
-    _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
-    _need_i32(what, positions=positions, token_seq=token_seq, page_indptr=page_indptr, page_ids=page_ids)
-    _need(positions.numel() >= n and token_seq.numel() >= n, f"{what}: a position and a request a token")
-    _need(0 <= rotary_dim <= head_dim and rotary_dim % 2 == 0, f"{what}: rotary_dim")
-    if rotary_dim:
-        _need(inv_freq is not None and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and inv_freq.numel() == rotary_dim // 2,
-              f"{what}: inv_freq must be float32 [rotary_dim/2]")
-    _check(_fn(_libs.get("cache8.cu"), "tkb_rope_kv8_write")(
-        _ptr(qkv), c_int(f32), _ptr(positions), _ptr(token_seq), _ptr(page_indptr), _ptr(page_ids), _ptr(inv_freq), _ptr(kcache),
-        _ptr(vcache), _ptr(k_scale), _ptr(v_scale), c_int(n), c_int(n_heads), c_int(n_kv_heads), c_int(head_dim), c_int(rotary_dim),
-        c_int(page_size), c_int(kcache.shape[0]), c_int(1 if write_cache else 0), _ptr(status), _stream()), what)
+    if not (qkv.dim() == 2 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and qkv.data_ptr() % 16 == 0):
+        raise KernelError(f"{what}: rows [q heads | k heads | v heads] x head size, contiguous, on a 16-byte boundary")
+    n = qkv.shape[0]
+    pages = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    _check_i32(what, positions, token_seq, page_indptr, page_ids)
+    if positions.numel() < n or token_seq.numel() < n:
+        raise KernelError(f"{what}: a position and a request a token")
+    if not (0 <= rotary_dim <= head_dim and rotary_dim % 2 == 0):
+        raise KernelError(f"{what}: an even number of each head's {head_dim} is rotated, not {rotary_dim}")
+    if rotary_dim and not (inv_freq is not None and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
+                           and inv_freq.numel() == rotary_dim // 2):
+        raise KernelError(f"{what}: inv_freq must be float32 [rotary_dim/2]")
+    _check(_entry("cache8.cu", "tkb_rope_kv8_write")(
+        qkv.data_ptr(), f32, positions.data_ptr(), token_seq.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
+        None if inv_freq is None else inv_freq.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, n_heads,
+        n_kv_heads, head_dim, rotary_dim, page_size, pages, 1 if write_cache else 0, status.data_ptr(), _stream()), what)
 
 
 def read_kv8(kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, pages: torch.Tensor,
              status: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that ``pages`` (int32 [n]) hold, as float32 [n, kv heads, page size, head size] each; zeros for an
     id that is negative or beyond the pool (the latter sets the status word's page bit)."""
+    what = "read_kv8"
     _need_cuda(kcache, vcache, k_scale, v_scale, pages, status)
-    _need(kcache.dim() == 4, "read_kv8: the cache is int8 [pages, kv heads, page size, head size]")
-    n_kv, ps, hd = kcache.shape[1:]
-    _check_cache("read_kv8", kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
-    _need_i32("read_kv8", pages=pages)
-    _need(ps * hd % 16 == 0, "read_kv8: page size times head size is a multiple of 16")
+    if kcache.dim() != 4 or kcache.shape[2] * kcache.shape[3] % 16:
+        raise KernelError(f"{what}: the cache is int8 [pages, kv heads, page size, head size], a page's codes of a head a multiple of 16")
+    _, n_kv, ps, hd = kcache.shape
+    pool = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
+    _check_i32(what, pages)
     n = pages.numel()
-    k = torch.empty((n, n_kv, ps, hd), dtype=torch.float32, device=kcache.device)
-    v = torch.empty_like(k)
-    _check(_fn(_libs.get("cache8.cu"), "tkb_read_kv8")(
-        _ptr(kcache), _ptr(vcache), _ptr(k_scale), _ptr(v_scale), _ptr(pages), _ptr(k), _ptr(v), c_int(n), c_int(n_kv), c_int(ps * hd),
-        c_int(kcache.shape[0]), _ptr(status), _stream()), "read_kv8")
+    out = torch.empty((2, n, n_kv, ps, hd), dtype=torch.float32, device=kcache.device)
+    k, v = out.unbind(0)
+    _check(_entry("cache8.cu", "tkb_read_kv8")(
+        kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, n_kv, ps * hd,
+        pool, status.data_ptr(), _stream()), what)
     return k, v
 
 
@@ -237,41 +247,45 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     _need_cuda(q, out, kcache, vcache, k_scale, v_scale, q_start, q_len, kv_len, page_indptr, page_ids, status)
     f32 = _is_f32(q.dtype)
     check_head_dim(head_dim)
-    _need(n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0 and page_size >= 1, f"{what}: heads in groups of a kv head")
+    if not (n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0 and page_size >= 1):
+        raise KernelError(f"{what}: heads in groups of a kv head")
     width = n_heads * head_dim
-    for t, name in ((q, "q"), (out, "out")):
-        _need(t.dim() == 2 and t.shape[1] >= width and t.stride(1) == 1 and t.dtype == q.dtype, f"{what}: {name} has rows of heads of one type")
-    _need(out.shape[0] >= q.shape[0], f"{what}: a row of out for every row of q")
-    _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
-    _need_i32(what, q_start=q_start, q_len=q_len, kv_len=kv_len, page_indptr=page_indptr, page_ids=page_ids)
+    if not (q.dim() == out.dim() == 2 and q.shape[1] >= width and out.shape[1] >= width and q.stride(1) == 1 and out.stride(1) == 1
+            and out.dtype == q.dtype and out.shape[0] >= q.shape[0]):
+        raise KernelError(f"{what}: rows of {n_heads} heads of {head_dim} in q and, of the same type, in out")
+    pool = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    _check_i32(what, q_start, q_len, kv_len, page_indptr, page_ids)
     n = q_len.numel()
-    _need(q_start.numel() >= n and kv_len.numel() >= n and page_indptr.numel() > n, f"{what}: a start, a length and pages for every request")
-    _need(window is None or window >= 1, f"{what}: a window of one key at least")
-    _need(scale > 0, f"{what}: scores are scaled by a positive number")
-    _need(max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n and (portions is None or portions >= 0), f"{what}: bounds")
+    if q_start.numel() < n or kv_len.numel() < n or page_indptr.numel() <= n:
+        raise KernelError(f"{what}: a start, a length and pages for every request")
+    if window is not None and window < 1:
+        raise KernelError(f"{what}: a window of one key at least")
+    if not scale > 0:
+        raise KernelError(f"{what}: scores are scaled by a positive number")
+    if not (max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n and (portions is None or portions >= 0)):
+        raise KernelError(f"{what}: bounds")
     T = q.shape[0]
     if n == 0 or T == 0:
         return
+    window = window or 0
     group = n_heads // n_kv_heads
     singles = min(single_tokens, T)
     exact = portions is None
     portions = (n - singles if exact else min(portions, n)) if max_q_len > 1 else 0
+    common = (q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
+              v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr())
     which, tokens, requests = 3, T, n
     if head_dim <= KV8_TC_MAX_DIM:
         # portions on the tcgen05 tensor cores, single tokens with their keys cut over the GPU
         if portions:
             _check(_entry("attention_kv8_tc.cu", "tkb_attn_kv8_tc", head_dim)(
-                q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
-                v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
-                n, portions, T - singles if exact else T, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0],
-                status.data_ptr(), _stream()), what)
+                *common, n, portions, T - singles if exact else T, n_heads, n_kv_heads, page_size, scale, window, pool, status.data_ptr(),
+                _stream()), what)
         if singles == 0:
             return
         which, tokens, requests = 1, singles, singles
     scratch = torch.empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group),),
                           dtype=torch.uint8, device=q.device)
     _check(_entry("attention_kv8.cu", "tkb_attn_kv8", head_dim)(
-        q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
-        v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
-        scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window or 0, kcache.shape[0], which,
+        *common, scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window, pool, which,
         status.data_ptr(), _stream()), what)
