@@ -371,9 +371,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_remote(uint32_t addr, int rank, uint32_t v) {
-  asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nst.shared::cluster.u32 [r], %2;\n}" ::"r"(addr), "r"(rank), "r"(v) : "memory");
+__device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
 }
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
 template <int NTOK, bool GATED, typename T>
 __global__ void __launch_bounds__(THREADS, 2)
@@ -383,6 +386,7 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   extern __shared__ unsigned char smem_raw[];
   constexpr int STAGES = FewCfg<NTOK>::STAGES, STAGE_BYTES = FewCfg<NTOK>::STAGE_BYTES, TMEM_COLS = FewCfg<NTOK>::TMEM_COLS;
   __shared__ __align__(8) uint64_t full_bar[STAGES], empty_bar[STAGES], acc_bar;
+  __shared__ float tok_scale[NTOK];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int failed;
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -451,22 +455,24 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   const int q = warp & 3, f = q * 32 + lane;  // an epilogue thread's channel of the block's
   const uint32_t t_addr = tmem_acc + ((uint32_t)(q * 32) << 16);
   bool ok = true;
+  float ts = 0.f;
   if (warp >= 2) {
     grid_dependency_wait();  // nothing is stored before the kernel ahead of this one has finished
+    // the tokens' scales to shared memory, on their way with the products
+    for (int i = threadIdx.x - 64; i < M; i += 128) tok_scale[i] = a_scale[i];
+    ts = n0 + f < N ? w_scale[n0 + f] : 0.f;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     ok = mbar_wait(&acc_bar, 0);
     tcgen05_fence_after();
     if (!ok) failed = 1;
   }
-  const float ts = warp >= 2 && n0 + f < N ? w_scale[n0 + f] : 0.f;
+  // A token's sum of this thread's channel: scaled and stored (gated: the up channel's value comes from eight lanes on).
+  T* const dst = out + (GATED ? ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7) : n0 + f);
+  const bool stores = GATED ? (lane & 8) == 0 && n0 + f + 8 < N : n0 + f < N;
   auto finish = [&](int m, uint32_t sum) {
-    // one token's sum of this thread's channel: scaled and stored (gated: the up channel's value comes from eight lanes on)
-    const float y = value_of(sum, a_scale[m] * ts);
-    if (!GATED) {
-      if (n0 + f < N) out[(long long)m * ldo + n0 + f] = from_float<T>(y);
-    } else {
-      const float up = __shfl_down_sync(0xffffffffu, y, 8);
-      if ((lane & 8) == 0 && n0 + f + 8 < N) out[(long long)m * ldo + ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7)] = from_float<T>(silu_mul_fast(y, up));
-    }
+    float y = value_of(sum, tok_scale[m] * ts);
+    if (GATED) y = silu_mul_fast(y, __shfl_down_sync(0xffffffffu, y, 8));
+    if (stores) dst[(long long)m * ldo] = from_float<T>(y);
   };
   if (parts == 1) {
     if (warp >= 2 && ok) {
@@ -480,27 +486,38 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
     }
   } else {
-    // token c belongs to part c % parts; its sums stand there as [c / parts][part][channel], where the ring was
+    // Tokens go to the parts in runs of `run`; a token's sums stand with its part as [place in the run][part][channel], where the ring was.
     uint32_t* sums = reinterpret_cast<uint32_t*>(ring);
+    const int run = (M + parts - 1) / parts;
     cluster_sync();  // every block's MMAs have read their stages
     if (warp >= 2 && ok) {
+      int owner = 0, at = 0;
+      uint32_t base = remote(smem_u32(&sums[part * BC + f]), 0);
 #pragma unroll 1
       for (int c0 = 0; c0 < NTOK && c0 < M; c0 += 16) {
         uint32_t r[16];
         tmem_ld16(t_addr + c0, r);
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const int c = c0 + i;
-          if (c < M) store_remote(smem_u32(&sums[((c / parts) * parts + part) * BC + f]), c % parts, r[i]);
+          if (c0 + i < M) {
+            store_cluster(base + at * (parts * BC * 4), r[i]);
+            if (++at == run) {
+              at = 0;
+              base = remote(smem_u32(&sums[part * BC + f]), ++owner < parts ? owner : 0);
+            }
+          }
         }
       }
     }
     cluster_sync();
     if (warp >= 2) {
-      for (int c = part; c < M; c += parts) {
+      const int first = part * run, n = min(run, M - first);
+#pragma unroll 2
+      for (int c = 0; c < n; c++) {
         uint32_t sum = 0;
-        for (int i = 0; i < parts; i++) sum += sums[((c / parts) * parts + i) * BC + f];
-        finish(c, sum);
+#pragma unroll
+        for (int i = 0; i < MAX_PARTS; i++) sum += i < parts ? sums[(c * parts + i) * BC + f] : 0u;
+        finish(first + c, sum);
       }
     }
   }
