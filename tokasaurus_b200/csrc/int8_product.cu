@@ -376,7 +376,11 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 template <int NTOK, bool GATED, typename T>
 __global__ void __launch_bounds__(THREADS, 2)
@@ -459,7 +463,7 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   if (warp >= 2) {
     grid_dependency_wait();  // nothing is stored before the kernel ahead of this one has finished
     // the tokens' scales to shared memory, on their way with the products
-    for (int i = threadIdx.x - 64; i < M; i += 128) tok_scale[i] = a_scale[i];
+    if (threadIdx.x - 64 < NTOK) tok_scale[threadIdx.x - 64] = threadIdx.x - 64 < M ? a_scale[threadIdx.x - 64] : 0.f;
     ts = n0 + f < N ? w_scale[n0 + f] : 0.f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
     ok = mbar_wait(&acc_bar, 0);
@@ -469,10 +473,12 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   // A token's sum of this thread's channel: scaled and stored (gated: the up channel's value comes from eight lanes on).
   T* const dst = out + (GATED ? ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7) : n0 + f);
   const bool stores = GATED ? (lane & 8) == 0 && n0 + f + 8 < N : n0 + f < N;
+  // (Only the store asks whether the token is one: sixteen results are worked out together.  With a branch around each, one waited for
+  // the other, 12,000 clocks for 64 gated tokens.)
   auto finish = [&](int m, uint32_t sum) {
     float y = value_of(sum, tok_scale[m] * ts);
     if (GATED) y = silu_mul_fast(y, __shfl_down_sync(0xffffffffu, y, 8));
-    if (stores) dst[(long long)m * ldo] = from_float<T>(y);
+    if (stores && m < M) dst[(long long)m * ldo] = from_float<T>(y);
   };
   if (parts == 1) {
     if (warp >= 2 && ok) {
@@ -481,45 +487,43 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         uint32_t r[16];
         tmem_ld16(t_addr + c0, r);
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (c0 + i < M) finish(c0 + i, r[i]);
+        for (int i = 0; i < 16; i++) finish(c0 + i, r[i]);
       }
     }
   } else {
-    // Tokens go to the parts in runs of `run`; a token's sums stand with its part as [place in the run][part][channel], where the ring was.
+    // Every block leaves its sums [token][channel] where its ring was (its own MMAs are through with it); each part adds up a run of
+    // tokens from all of them.
     uint32_t* sums = reinterpret_cast<uint32_t*>(ring);
-    const int run = (M + parts - 1) / parts;
-    cluster_sync();  // every block's MMAs have read their stages
     if (warp >= 2 && ok) {
-      int owner = 0, at = 0;
-      uint32_t base = remote(smem_u32(&sums[part * BC + f]), 0);
 #pragma unroll 1
       for (int c0 = 0; c0 < NTOK && c0 < M; c0 += 16) {
         uint32_t r[16];
         tmem_ld16(t_addr + c0, r);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          if (c0 + i < M) {
-            store_cluster(base + at * (parts * BC * 4), r[i]);
-            if (++at == run) {
-              at = 0;
-              base = remote(smem_u32(&sums[part * BC + f]), ++owner < parts ? owner : 0);
-            }
-          }
-        }
+        for (int i = 0; i < 16; i++) sums[(c0 + i) * BC + f] = r[i];
       }
     }
     cluster_sync();
     if (warp >= 2) {
-      const int first = part * run, n = min(run, M - first);
-#pragma unroll 2
-      for (int c = 0; c < n; c++) {
-        uint32_t sum = 0;
+      const int run = (M + parts - 1) / parts, end = min(M, (part + 1) * run);
+      const uint32_t mine = smem_u32(&sums[f]);
+#pragma unroll 1
+      for (int c = part * run; c < end; c += 4) {
+        uint32_t x[4][MAX_PARTS];
 #pragma unroll
-        for (int i = 0; i < MAX_PARTS; i++) sum += i < parts ? sums[(c * parts + i) * BC + f] : 0u;
-        finish(first + c, sum);
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int p = 0; p < MAX_PARTS; p++) x[i][p] = p < parts ? load_cluster(remote(mine + min(c + i, end - 1) * (BC * 4), p)) : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          uint32_t sum = 0;
+#pragma unroll
+          for (int p = 0; p < MAX_PARTS; p++) sum += x[i][p];
+          finish(min(c + i, end - 1), sum);  // (the last one again and again behind the end)
+        }
       }
     }
+    cluster_sync();  // (no block leaves while others read its sums)
   }
   if (warp >= 2) tcgen05_fence_before();
   __syncthreads();
@@ -546,7 +550,7 @@ int launch_few(const void* a, long long lda, const float* a_scale, const void* w
   if (parts < 1) parts = 1;
   const int per = (kblocks + parts - 1) / parts;
   parts = (kblocks + per - 1) / per;
-  static_assert((NTOK + MAX_PARTS) * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
+  static_assert(NTOK * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles, parts);
   cfg.blockDim = dim3(THREADS);
