@@ -9,7 +9,8 @@ A request holds one block table per group.  Pages are handed out as the request'
 them (tokasaurus/manager/allocator.py:254-296 ``allocate_up_to_length``), given back when the
 request ends (tokasaurus/manager/types.py:324-338 ``deallocate``) or, in a group whose mixer sees
 only a window of keys, as soon as the window has moved past them.  Device layout of a group:
-``[layer call, k|v, page, kv head, slot in page, head_dim]``.
+``[layer call, k|v, page, kv head, slot in page, head_dim]``; a group that holds 8-bit codes has float32 scales
+``[layer call, k|v, page, kv head]`` beside them.
 """
 
 from __future__ import annotations
@@ -34,8 +35,12 @@ class CacheGroup:
     entries: list[int]
     allocator: PageAllocator
     storage: torch.Tensor | None = None  # [len(entries), planes, pages, kv heads, page_size, head_dim]
+    scales: torch.Tensor | None = None   # float32 [len(entries), planes, pages, kv heads] of a group that holds 8-bit codes
 
     def bytes_per_token(self, element_size: int) -> int:
+        """Without the scales of a group that holds 8-bit codes (four bytes a page, plane and kv head)."""
+        if self.need.eight_bits:
+            element_size = 1
         return self.need.planes * len(self.entries) * self.need.n_kv_heads * self.need.head_dim * element_size
 
 
@@ -46,6 +51,8 @@ class PagedLayerCache:
     v: torch.Tensor | None
     page_size: int
     writable: bool = True
+    k_scale: torch.Tensor | None = None  # float32 [pages, kv heads], where k and v are 8-bit codes
+    v_scale: torch.Tensor | None = None
 
 
 @dataclass
@@ -127,7 +134,10 @@ class CacheManager:
             for g in self.groups:
                 n = g.need
                 g.storage = torch.zeros((len(g.entries), n.planes, g.allocator.num_pages, n.n_kv_heads, page_size, n.head_dim),
-                                        dtype=dtype, device=self.device)
+                                        dtype=torch.int8 if n.eight_bits else dtype, device=self.device)
+                if n.eight_bits:
+                    g.scales = torch.zeros((len(g.entries), n.planes, g.allocator.num_pages, n.n_kv_heads), dtype=torch.float32,
+                                           device=self.device)
             for entry, need in self._state_need.items():
                 self._state[entry] = torch.zeros((max_requests, *need.shape), dtype=_DTYPES[need.dtype],
                                                  device=self.device)
@@ -148,7 +158,8 @@ class CacheManager:
 
     def device_bytes_by_group(self) -> list[int]:
         """Bytes of key/value storage of each cache group (0 where the manager keeps books only)."""
-        return [g.storage.numel() * g.storage.element_size() if g.storage is not None else 0 for g in self.groups]
+        held = [[t for t in (g.storage, g.scales) if t is not None] for g in self.groups]
+        return [sum(t.numel() * t.element_size() for t in ts) for ts in held]
 
     def num_free_pages(self) -> list[int]:
         return [g.allocator.num_free for g in self.groups]
@@ -240,9 +251,11 @@ class CacheManager:
         if entry in self._entry_group:
             g, i = self._entry_group[entry]
             st = self.groups[g].storage
+            sc = self.groups[g].scales
             return PagedLayerCache(g, st[i, 0] if st is not None else None,
                                    st[i, 1] if st is not None and st.shape[1] > 1 else None,
-                                   self.page_size, writable)
+                                   self.page_size, writable, sc[i, 0] if sc is not None else None,
+                                   sc[i, 1] if sc is not None and sc.shape[1] > 1 else None)
         if entry in self._state_need:
             return StateLayerCache(self._state.get(entry), writable)
         return None

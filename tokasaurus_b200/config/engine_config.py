@@ -47,6 +47,8 @@ class EngineConfig:
     # --- this engine's own options ---
     random_weights: int | None = None  # seed: build weights from the configuration instead of reading them
     device: str = "cuda:0"
+    linear_dtype: str | None = None    # "int8": the blocks' matrices in 8 bits, tokens brought to 8 bits on the way in (None: as dtype)
+    kv_cache_dtype: str | None = None  # "int8": keys and values in 8 bits with a scale a page and kv head (None: as dtype)
 
     def kv_cache_num_blocks(self) -> int:
         # tokasaurus/common_types.py:130-132
@@ -59,6 +61,9 @@ class EngineConfig:
     def finalize(self, max_position_embeddings: int | None = None) -> "EngineConfig":
         if self.dtype not in ("bfloat16", "float32"):
             raise OptionError(f"dtype={self.dtype!r}: this engine runs 'bfloat16' or 'float32'")
+        for name in ("linear_dtype", "kv_cache_dtype"):
+            if getattr(self, name) not in (None, "int8"):
+                raise OptionError(f"{name}={getattr(self, name)!r}: 'int8', or nothing for the engine's dtype")
         for name in ("page_size", "kv_cache_num_tokens", "max_tokens_per_forward", "max_seqs_per_forward",
                      "prefill_round_up_multiple", "cudagraph_step", "cudagraph_max_size"):
             if getattr(self, name) <= 0:

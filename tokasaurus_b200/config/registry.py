@@ -25,6 +25,7 @@ class Architecture:
     parse_config: Callable[[dict[str, Any]], Any]
     build_model: Callable[[Any], Any]
     model_types: tuple[str, ...] = ()
+    eight_bits: bool = False  # ``build_model`` takes ``int8_linears`` and ``int8_cache``
 
 
 _BY_NAME: dict[str, Architecture] = {}
@@ -37,11 +38,13 @@ def register_architecture(
     build_model: Callable[[Any], Any],
     model_types: tuple[str, ...] = (),
     replace: bool = False,
+    eight_bits: bool = False,
 ) -> Architecture:
-    """Add an architecture.  ``name`` is what config.json lists under ``architectures``."""
+    """Add an architecture.  ``name`` is what config.json lists under ``architectures``.  ``eight_bits``: its ``build_model``
+    takes ``int8_linears=`` and ``int8_cache=``."""
     if name in _BY_NAME and not replace:
         raise ValueError(f"architecture {name!r} is already registered")
-    arch = Architecture(name, parse_config, build_model, tuple(model_types))
+    arch = Architecture(name, parse_config, build_model, tuple(model_types), eight_bits)
     _BY_NAME[name] = arch
     for mt in model_types:
         _BY_MODEL_TYPE[mt] = arch

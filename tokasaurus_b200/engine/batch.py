@@ -72,6 +72,8 @@ class StepContext:
         self.n_seqs = int(host.seq_slot.shape[0])
         # every request brings exactly one token (a decode step): kernels that fuse across a token's row may run
         self.single_token_step = self.n_tokens == self.n_seqs and bool((host.seq_q_len == 1).all())
+        # recorded as a graph of a decode step: it is replayed for steps of single tokens only (padded requests bring none)
+        self.decode_graph = False
         self.some_single_token = bool((host.seq_q_len == 1).any())
         self.all_rows_wanted = (
             host.logit_rows.shape[0] == self.n_tokens

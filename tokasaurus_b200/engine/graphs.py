@@ -175,6 +175,8 @@ class DecodeGraphs:
             # a graph of a padded mixed step is replayed for other steps of its shape: no kernel in it may rest on
             # every request bringing one token, even if the step it is recorded from happens to be such a step
             ctx.single_token_step = False
+        else:
+            ctx.decode_graph = True
         runner.last_upload_bytes = slot["stager"].bytes_last_upload
         runner.last_context = ctx
         if slot["graph"] is None:

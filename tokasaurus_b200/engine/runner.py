@@ -15,7 +15,7 @@ from typing import Any, Sequence
 import torch
 
 from tokasaurus_b200.cache.manager import CacheManager
-from tokasaurus_b200.config.engine_config import EngineConfig, parse_rope_scaling_override
+from tokasaurus_b200.config.engine_config import EngineConfig, OptionError, parse_rope_scaling_override
 from tokasaurus_b200.config.model_config import read_config_json, read_eos_token_ids
 from tokasaurus_b200.config.registry import lookup_architecture
 from tokasaurus_b200.engine.batch import Stager, StepContext, StepEntry, build_host_batch
@@ -57,16 +57,21 @@ class ModelRunner:
         self.config_dict = config_dict
         self.arch = lookup_architecture(config_dict)
         self.model_config = self.arch.parse_config(config_dict)
-        self.model = self.arch.build_model(self.model_config)
+        config.finalize(getattr(self.model_config, "max_position_embeddings", None))
+        eight = {}
+        if config.linear_dtype is not None or config.kv_cache_dtype is not None:
+            if not self.arch.eight_bits:
+                raise OptionError(f"linear_dtype and kv_cache_dtype: {self.arch.name} runs in the engine's dtype only")
+            eight = dict(int8_linears=config.linear_dtype == "int8", int8_cache=config.kv_cache_dtype == "int8")
+        self.model = self.arch.build_model(self.model_config, **eight)
         self.eos_token_ids = (
             read_eos_token_ids(config.model, config_dict) if config.model else
             tuple([config_dict["eos_token_id"]] if isinstance(config_dict.get("eos_token_id"), int)
                   else config_dict.get("eos_token_id") or ())
         )
-        config.finalize(getattr(self.model_config, "max_position_embeddings", None))
 
         needs = self.model.cache_entries()
-        head_dims = sorted({n.head_dim for n in needs.values() if isinstance(n, PagedCacheNeed) and n.planes == 2})
+        head_dims = sorted({n.head_dim for n in needs.values() if isinstance(n, PagedCacheNeed) and n.planes == 2 and not n.eight_bits})
         ops.prepare(head_dims, self.rt.dtype)
         ops.prepare_modules(self.model.kernel_modules("float32" if self.rt.dtype == torch.float32 else "bfloat16"))
 

@@ -10,11 +10,15 @@ llama.py:842-845).
 
 from __future__ import annotations
 
+from functools import partial
+
 from tokasaurus_b200.config.model_config import LlamaConfig
 from tokasaurus_b200.config.registry import register_architecture
 from tokasaurus_b200.parts import (
     DecoderModel,
     GatedMLP,
+    Int8GatedMLP,
+    Int8PagedAttention,
     OutputHead,
     PagedAttention,
     PreNormBlock,
@@ -24,7 +28,11 @@ from tokasaurus_b200.parts import (
 )
 
 
-def build_llama(cfg: LlamaConfig) -> DecoderModel:
+def build_llama(cfg: LlamaConfig, int8_linears: bool = False, int8_cache: bool = False) -> DecoderModel:
+    """``int8_linears``: the blocks' matrices and the tokens that meet them in 8 bits; ``int8_cache``: keys and values in 8
+    bits (``parts.int8``)."""
+    attention = partial(Int8PagedAttention, int8_linears=int8_linears, int8_cache=int8_cache) if int8_linears or int8_cache else PagedAttention
+    mlp = Int8GatedMLP if int8_linears else GatedMLP
     H, hd = cfg.hidden_size, cfg.head_dim
     rs = cfg.rope_scaling
     if rs is not None and rs.rope_type == "llama3":
@@ -38,14 +46,14 @@ def build_llama(cfg: LlamaConfig) -> DecoderModel:
         blocks.append(
             PreNormBlock(
                 mixer_norm=RMSNorm(H, cfg.rms_norm_eps, f"{p}.input_layernorm.weight"),
-                mixer=PagedAttention(
+                mixer=attention(
                     H, cfg.num_attention_heads, cfg.num_key_value_heads, hd, position,
                     q_name=f"{p}.self_attn.q_proj.weight", k_name=f"{p}.self_attn.k_proj.weight",
                     v_name=f"{p}.self_attn.v_proj.weight", o_name=f"{p}.self_attn.o_proj.weight",
                 ),
                 ffn_norm=RMSNorm(H, cfg.rms_norm_eps, f"{p}.post_attention_layernorm.weight"),
-                ffn=GatedMLP(H, cfg.intermediate_size, gate_name=f"{p}.mlp.gate_proj.weight",
-                             up_name=f"{p}.mlp.up_proj.weight", down_name=f"{p}.mlp.down_proj.weight"),
+                ffn=mlp(H, cfg.intermediate_size, gate_name=f"{p}.mlp.gate_proj.weight",
+                        up_name=f"{p}.mlp.up_proj.weight", down_name=f"{p}.mlp.down_proj.weight"),
             )
         )
     embed_name = "model.embed_tokens.weight"
@@ -62,4 +70,5 @@ def build_llama(cfg: LlamaConfig) -> DecoderModel:
     )
 
 
-register_architecture("LlamaForCausalLM", LlamaConfig.from_dict, build_llama, model_types=("llama",), replace=True)
+register_architecture("LlamaForCausalLM", LlamaConfig.from_dict, build_llama, model_types=("llama",), replace=True,
+                      eight_bits=True)

@@ -16,6 +16,7 @@ from tokasaurus_b200.parts.conv import ShortConv  # noqa: F401
 from tokasaurus_b200.parts.rope import NoPositionEncoding, RotaryEncoding, SinusoidalPositions  # noqa: F401
 from tokasaurus_b200.parts.attention import PagedAttention  # noqa: F401
 from tokasaurus_b200.parts.mlp import ClampedGLU, GatedMLP, GeluMLP, PolyNormMLP, RoutedExperts, SquaredReluMLP  # noqa: F401
+from tokasaurus_b200.parts.int8 import Int8GatedMLP, Int8PagedAttention  # noqa: F401
 from tokasaurus_b200.parts.recurrent import (  # noqa: F401
     DecayedLinearAttention,
     GatedLinearAttention,

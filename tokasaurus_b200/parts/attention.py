@@ -369,6 +369,14 @@ class PagedAttention(AttentionPlanning, Mixer):
                               cache.k, cache.v, nh, nkv, hd, rot, cache.page_size, cache.writable, ctx.status,
                               bias=self.qkv_bias, qk_norm=self.qk_norm, norm_eps=self.norm_eps)
             project = ops.linear
+        return project(self.attend(ctx, qkv, cache, out_rows), self.w_o)
+
+    def attend(self, ctx, qkv, cache, out_rows=None):
+        """The attention of the step's tokens, whose rotated queries are the first columns of ``qkv`` and whose keys and
+        values are in the cache: [T or len(out_rows), n_heads * head_dim]."""
+        h, T = qkv, qkv.shape[0]
+        hd, nh, nkv = self.head_dim, self.n_heads, self.n_kv_heads
+        tables = ctx.tables[cache.group]
         plan = ctx.plans.get(self.plan_key()) if h.dtype == torch.bfloat16 else None
         if plan is not None and out_rows is not None and out_rows is ctx.logit_rows and "row_items" in plan:
             # only some rows are wanted (the last block of a step): one split-key query per wanted row
@@ -385,7 +393,7 @@ class PagedAttention(AttentionPlanning, Mixer):
                                 self.scale, self.window, out_row_of=plan["row_index"],
                                 item_entry=plan["row_item_entry"], tma=bool(counts[6]), status=ctx.status,
                                 item_order=plan["row_item_order"] if caps or not counts[10] & ops.ITEMS_LISTED else None)
-            return project(attn, self.w_o)
+            return attn
         if plan is None or out_rows is not None:
             # float32, or only some rows are wanted: the FP32-pipe kernel
             n_rows = T if out_rows is None else out_rows.numel()
@@ -393,7 +401,7 @@ class PagedAttention(AttentionPlanning, Mixer):
             ops.attn_paged(qkv, qkv.shape[1], attn, cache.k, cache.v, ctx.token_seq, ctx.positions, tables.indptr,
                            tables.page_ids, out_rows, n_rows, nh, nkv, hd, cache.page_size, self.scale, self.window,
                            ctx.status)
-            return project(attn, self.w_o)
+            return attn
         attn = torch.empty((T, nh * hd), dtype=h.dtype, device=h.device)
         caps = ctx.plan_caps.get(self.plan_key()) if ctx.plan_caps else None
         counts = ctx.host_plans[self.plan_key()]["counts"]
@@ -415,4 +423,4 @@ class PagedAttention(AttentionPlanning, Mixer):
             ops.attn_prefill_mma(qkv, attn, cache.k, cache.v, ctx.seq_q_start, ctx.seq_q_len, ctx.seq_kv_len,
                                  tables.indptr, tables.page_ids, plan["tiles"], c[2:3], tiles_cap, nh, nkv, hd,
                                  cache.page_size, self.scale, self.window, ctx.status)
-        return project(attn, self.w_o)
+        return attn

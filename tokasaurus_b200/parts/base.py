@@ -51,7 +51,8 @@ class PagedCacheNeed:
     values, 1 for a mixer that keeps one row a token (a latent from which it makes both).  ``keep_first``: with a
     window, the request's first so many keys are read by every later query too: their pages stay.  ``chunked``: the
     window does not slide; the sequence is cut into chunks of ``window`` positions, counted from position 0, and a query
-    reads the keys of its own chunk only (never more than the sliding window would let it see)."""
+    reads the keys of its own chunk only (never more than the sliding window would let it see).  ``eight_bits``: rows are
+    held as 8-bit codes with a float32 scale a page, plane and kv head."""
 
     n_kv_heads: int
     head_dim: int
@@ -59,6 +60,7 @@ class PagedCacheNeed:
     planes: int = 2
     keep_first: int = 0
     chunked: bool = False
+    eight_bits: bool = False
 
     def first_visible(self, position: int) -> int:
         """The first key that a query at ``position`` or any later one reads (kept first keys aside)."""
