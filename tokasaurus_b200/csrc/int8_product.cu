@@ -354,7 +354,8 @@ constexpr int W8_BYTES = BC * BK8;     // 16 KiB
 
 template <int NTOK> struct FewCfg {
   static constexpr int STAGE_BYTES = W8_BYTES + NTOK * BK8;
-  static constexpr int STAGES = NTOK >= 128 ? 3 : NTOK >= 64 ? 4 : 5;  // two blocks an SM
+  static constexpr int BLOCKS = NTOK > 128 ? 1 : 2;  // an SM
+  static constexpr int STAGES = NTOK > 128 ? 4 : NTOK == 128 ? 3 : NTOK >= 64 ? 4 : 5;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
   static constexpr int TMEM_COLS = NTOK < 32 ? 32 : NTOK;
 };
@@ -376,16 +377,14 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 template <int NTOK, bool GATED, typename T>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, FewCfg<NTOK>::BLOCKS)
 product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ a_scale,
-                   const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int M, int N, int K, int kblocks_per_part,
+                   const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int all_tokens, int N, int K, int kblocks_per_part,
                    int weights_ready, int* __restrict__ status) {
   extern __shared__ unsigned char smem_raw[];
   constexpr int STAGES = FewCfg<NTOK>::STAGES, STAGE_BYTES = FewCfg<NTOK>::STAGE_BYTES, TMEM_COLS = FewCfg<NTOK>::TMEM_COLS;
@@ -395,7 +394,8 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   __shared__ int failed;
   unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * BC;
+  const int n0 = blockIdx.x * BC, m0 = blockIdx.z * NTOK;
+  const int M = min(NTOK, all_tokens - m0);        // tokens of this tile
   const int part = blockIdx.y, parts = gridDim.y;  // a cluster is all parts of a tile
   const int kb_begin = part * kblocks_per_part;
   const int nkb = max(0, min(kblocks_per_part, (K + BK8 - 1) / BK8 - kb_begin));
@@ -432,13 +432,13 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (lane == 0) {
       grid_dependency_wait();
       for (int kb = 0; kb < first; kb++)
-        tma_load_2d(ring + kb * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[kb], (kb_begin + kb) * BK8, 0);
+        tma_load_2d(ring + kb * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[kb], (kb_begin + kb) * BK8, m0);
       for (int kb = STAGES; kb < nkb; kb++) {
         const int s = kb % STAGES;
         if (!mbar_wait(&empty_bar[s], ((kb / STAGES) - 1) & 1)) { failed = 1; break; }
         mbar_expect_tx(&full_bar[s], STAGE_BYTES);
         tma_load_2d(ring + s * STAGE_BYTES, &map_w, &full_bar[s], (kb_begin + kb) * BK8, n0);
-        tma_load_2d(ring + s * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[s], (kb_begin + kb) * BK8, 0);
+        tma_load_2d(ring + s * STAGE_BYTES + W8_BYTES, &map_a, &full_bar[s], (kb_begin + kb) * BK8, m0);
       }
     }
   } else if (warp == 1) {
@@ -463,7 +463,7 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   if (warp >= 2) {
     grid_dependency_wait();  // nothing is stored before the kernel ahead of this one has finished
     // the tokens' scales to shared memory, on their way with the products
-    if (threadIdx.x - 64 < NTOK) tok_scale[threadIdx.x - 64] = threadIdx.x - 64 < M ? a_scale[threadIdx.x - 64] : 0.f;
+    for (int m = threadIdx.x - 64; m < NTOK; m += 128) tok_scale[m] = m < M ? a_scale[m0 + m] : 0.f;
     ts = n0 + f < N ? w_scale[n0 + f] : 0.f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
     ok = mbar_wait(&acc_bar, 0);
@@ -471,7 +471,7 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (!ok) failed = 1;
   }
   // A token's sum of this thread's channel: scaled and stored (gated: the up channel's value comes from eight lanes on).
-  T* const dst = out + (GATED ? ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7) : n0 + f);
+  T* const dst = out + m0 * ldo + (GATED ? ((n0 + q * 32 + (lane & 16)) >> 1) + (lane & 7) : n0 + f);
   const bool stores = GATED ? (lane & 8) == 0 && n0 + f + 8 < N : n0 + f < N;
   // (Only the store asks whether the token is one: sixteen results are worked out together.  With a branch around each, one waited for
   // the other, 12,000 clocks for 64 gated tokens.)
@@ -491,39 +491,40 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
     }
   } else {
-    // Every block leaves its sums [token][channel] where its ring was (its own MMAs are through with it); each part adds up a run of
-    // tokens from all of them.
-    uint32_t* sums = reinterpret_cast<uint32_t*>(ring);
+    // Each part adds up a run of the tokens, in fours: every block writes its sums of them, [part][four tokens][channel][token], into that
+    // part's shared memory, where the ring was.
+    cluster_sync();  // every part's MMAs are through with its ring
+    const int fours = (M + 3) >> 2, run = (fours + parts - 1) / parts;
+    const uint32_t slot = smem_u32(ring) + (part * run * BC + f) * 16;
     if (warp >= 2 && ok) {
+      int owner = 0, at = 0;
 #pragma unroll 1
       for (int c0 = 0; c0 < NTOK && c0 < M; c0 += 16) {
         uint32_t r[16];
         tmem_ld16(t_addr + c0, r);
 #pragma unroll
-        for (int i = 0; i < 16; i++) sums[(c0 + i) * BC + f] = r[i];
+        for (int i = 0; i < 4; i++) {
+          if (c0 + 4 * i < M) store_cluster(remote(slot + at * (BC * 16), owner), r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+          if (++at == run) at = 0, owner++;
+        }
       }
     }
     cluster_sync();
     if (warp >= 2) {
-      const int run = (M + parts - 1) / parts, end = min(M, (part + 1) * run);
-      const uint32_t mine = smem_u32(&sums[f]);
+      const uint4* mine = reinterpret_cast<const uint4*>(ring) + f;
+      const int end = min(run, fours - part * run);
 #pragma unroll 1
-      for (int c = part * run; c < end; c += 4) {
-        uint32_t x[4][MAX_PARTS];
+      for (int c = 0; c < end; c++) {
+        uint4 x[MAX_PARTS];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int p = 0; p < MAX_PARTS; p++) x[p] = p < parts ? mine[(p * run + c) * BC] : make_uint4(0, 0, 0, 0);
+        uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int p = 0; p < MAX_PARTS; p++) x[i][p] = p < parts ? load_cluster(remote(mine + min(c + i, end - 1) * (BC * 4), p)) : 0u;
+        for (int p = 0; p < MAX_PARTS; p++) sum[0] += x[p].x, sum[1] += x[p].y, sum[2] += x[p].z, sum[3] += x[p].w;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          uint32_t sum = 0;
-#pragma unroll
-          for (int p = 0; p < MAX_PARTS; p++) sum += x[i][p];
-          finish(min(c + i, end - 1), sum);  // (the last one again and again behind the end)
-        }
+        for (int i = 0; i < 4; i++) finish(4 * (part * run + c) + i, sum[i]);
       }
     }
-    cluster_sync();  // (no block leaves while others read its sums)
   }
   if (warp >= 2) tcgen05_fence_before();
   __syncthreads();
@@ -544,15 +545,16 @@ int launch_few(const void* a, long long lda, const float* a_scale, const void* w
   CUtensorMap map_a, map_w;
   if ((rc = make_map8(&map_w, w, N, K, ldw, BC)) || (rc = make_map8(&map_a, a, M, K, lda, NTOK))) return rc;
   const int tiles = (N + BC - 1) / BC, kblocks = (K + BK8 - 1) / BK8;
-  int parts = sm_count() / tiles;
+  const int token_tiles = (M + NTOK - 1) / NTOK;
+  int parts = sm_count() / (tiles * token_tiles);
   if (parts > MAX_PARTS) parts = MAX_PARTS;
   if (parts > kblocks / 2) parts = kblocks / 2;
   if (parts < 1) parts = 1;
   const int per = (kblocks + parts - 1) / parts;
   parts = (kblocks + per - 1) / per;
-  static_assert(NTOK * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
+  static_assert((NTOK + 4 * MAX_PARTS) * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles, parts);
+  cfg.gridDim = dim3(tiles, parts, token_tiles);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = st;
@@ -576,6 +578,8 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
   if (M <= 32) return launch_few<32, GATED, T>(TKB_ARGS);
   if (M <= 64) return launch_few<64, GATED, T>(TKB_ARGS);
   if (M <= 128) return launch_few<128, GATED, T>(TKB_ARGS);
+  const long long few_tiles = (long long)((N + BC - 1) / BC) * ((M + 255) / 256);
+  if (2 * few_tiles <= sm_count()) return launch_few<256, GATED, T>(TKB_ARGS);
   if (N >= 256) return launch_many<256, GATED, T>(TKB_ARGS);
   return launch_many<128, GATED, T>(TKB_ARGS);
 #undef TKB_ARGS
