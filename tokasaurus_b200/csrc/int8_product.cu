@@ -354,8 +354,7 @@ constexpr int W8_BYTES = BC * BK8;     // 16 KiB
 
 template <int NTOK> struct FewCfg {
   static constexpr int STAGE_BYTES = W8_BYTES + NTOK * BK8;
-  static constexpr int BLOCKS = NTOK > 128 ? 1 : 2;  // an SM
-  static constexpr int STAGES = NTOK > 128 ? 4 : NTOK == 128 ? 3 : NTOK >= 64 ? 4 : 5;
+  static constexpr int STAGES = NTOK >= 128 ? 3 : NTOK >= 64 ? 4 : 5;  // two blocks an SM
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;
   static constexpr int TMEM_COLS = NTOK < 32 ? 32 : NTOK;
 };
@@ -382,7 +381,7 @@ __device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t a, uint32_
 }
 
 template <int NTOK, bool GATED, typename T>
-__global__ void __launch_bounds__(THREADS, FewCfg<NTOK>::BLOCKS)
+__global__ void __launch_bounds__(THREADS, 2)
 product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ a_scale,
                    const float* __restrict__ w_scale, T* __restrict__ out, long long ldo, int all_tokens, int N, int K, int kblocks_per_part,
                    int weights_ready, int* __restrict__ status) {
@@ -514,15 +513,21 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       const uint4* mine = reinterpret_cast<const uint4*>(ring) + f;
       const int end = min(run, fours - part * run);
 #pragma unroll 1
-      for (int c = 0; c < end; c++) {
-        uint4 x[MAX_PARTS];
+      for (int c = 0; c < end; c += 4) {
+        uint4 sum[4] = {};
+#pragma unroll 2
+        for (int p = 0; p < parts; p++)
 #pragma unroll
-        for (int p = 0; p < MAX_PARTS; p++) x[p] = p < parts ? mine[(p * run + c) * BC] : make_uint4(0, 0, 0, 0);
-        uint32_t sum[4] = {0, 0, 0, 0};
+          for (int i = 0; i < 4; i++) {
+            const uint4 x = mine[(p * run + min(c + i, end - 1)) * BC];
+            sum[i].x += x.x, sum[i].y += x.y, sum[i].z += x.z, sum[i].w += x.w;
+          }
 #pragma unroll
-        for (int p = 0; p < MAX_PARTS; p++) sum[0] += x[p].x, sum[1] += x[p].y, sum[2] += x[p].z, sum[3] += x[p].w;
-#pragma unroll
-        for (int i = 0; i < 4; i++) finish(4 * (part * run + c) + i, sum[i]);
+        for (int i = 0; i < 4; i++) {
+          if (c + i >= end) break;
+          const int m = 4 * (part * run + c + i);
+          finish(m, sum[i].x), finish(m + 1, sum[i].y), finish(m + 2, sum[i].z), finish(m + 3, sum[i].w);
+        }
       }
     }
   }
@@ -537,21 +542,14 @@ product_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
 template <int NTOK, bool GATED, typename T>
 int launch_few(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
-               long long ldo, int M, int N, int K, int weights_ready, int* status, cudaStream_t st) {
+               long long ldo, int M, int N, int K, int parts, int per, int weights_ready, int* status, cudaStream_t st) {
   static SharedMemoryRequest ask;
   constexpr int SMEM = FewCfg<NTOK>::SMEM_BYTES;
   int rc = ask({{(const void*)product_few_kernel<NTOK, GATED, T>, SMEM}});
   if (rc) return rc;
   CUtensorMap map_a, map_w;
   if ((rc = make_map8(&map_w, w, N, K, ldw, BC)) || (rc = make_map8(&map_a, a, M, K, lda, NTOK))) return rc;
-  const int tiles = (N + BC - 1) / BC, kblocks = (K + BK8 - 1) / BK8;
-  const int token_tiles = (M + NTOK - 1) / NTOK;
-  int parts = sm_count() / (tiles * token_tiles);
-  if (parts > MAX_PARTS) parts = MAX_PARTS;
-  if (parts > kblocks / 2) parts = kblocks / 2;
-  if (parts < 1) parts = 1;
-  const int per = (kblocks + parts - 1) / parts;
-  parts = (kblocks + per - 1) / per;
+  const int tiles = (N + BC - 1) / BC, token_tiles = (M + NTOK - 1) / NTOK;
   static_assert((NTOK + 4 * MAX_PARTS) * BC * 4 <= FewCfg<NTOK>::STAGES * FewCfg<NTOK>::STAGE_BYTES, "the sums go through the ring's memory");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles, parts, token_tiles);
@@ -570,16 +568,50 @@ int launch_few(const void* a, long long lda, const float* a_scale, const void* w
   return (int)cudaLaunchKernelEx(&cfg, product_few_kernel<NTOK, GATED, T>, map_w, map_a, a_scale, w_scale, (T*)out, ldo, M, N, K, per, weights_ready, status);
 }
 
+// Which product, tile and parts of K: the least estimate of clocks.  What these products wait for is codes coming into shared
+// memory: 60 bytes a clock where an SM has the large tile or two blocks of the other product, 40 where it has one block of that.
+// Parts' sums go to one another at 13 bytes a clock.  The constants are a fit to 1,031 measured times (1 to 1,024 tokens, eleven
+// matrices of 512 to 128,256 channels, every tile and number of parts): what this picks takes 1.3 % longer on average than the
+// fastest of all, 12 % at worst.  (One tile of the tokens' size and as many parts as SMs allow took 35 % longer at 128 tokens x
+// 4,096 x 6,144 and 4 times as long at 333 x 1,001 x 509.)
+struct Plan {
+  int tokens;      // of the tokens' tile; 0: the product for many tokens
+  int parts, per;  // blocks that share K, boxes of K each
+};
+Plan plan(int M, int N, int K) {
+  const long long n_sms = sm_count(), kblocks = (K + BK8 - 1) / BK8, tiles_n = (N + BC - 1) / BC;
+  const long long cluster_slots = n_sms * 9 / 10;  // clusters do not fill every group of SMs
+  auto rounds = [](long long blocks, long long slots) { return (blocks + slots - 1) / slots; };
+  const int wide = N >= 256 ? 256 : 128;
+  Plan best = {0, 1, (int)kblocks};
+  double least = rounds((long long)((N + wide - 1) / wide) * ((M + BM - 1) / BM), n_sms) * ((BM + wide) * BK8 / 60.0 * kblocks + 3000.0);
+  for (int tokens = 16; tokens <= 128; tokens *= 2) {
+    const long long tiles = tiles_n * ((M + tokens - 1) / tokens);
+    if (tiles > 65535) continue;
+    for (int parts = 1; parts <= MAX_PARTS && (parts == 1 || (parts * 2 <= kblocks + 1 && tiles * parts <= 2 * n_sms)); parts++) {
+      const long long per = (kblocks + parts - 1) / parts, used = (kblocks + per - 1) / per;
+      const long long r = rounds(tiles * used, used == 1 ? n_sms : cluster_slots);
+      double clocks = r * ((double)(BC + tokens) * BK8 * per / (r == 1 ? 40 : 60) + 20.0 * tokens / used) + 300.0 * used;
+      if (used > 1) clocks += r * (tokens * BC * 4 / 13.0);
+      if (clocks < least) least = clocks, best = {tokens, (int)used, (int)per};
+    }
+    if (tokens >= M) break;
+  }
+  return best;
+}
+
 template <bool GATED, typename T>
 int product(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
             long long ldo, int M, int N, int K, int weights_ready, int* status, cudaStream_t st) {
 #define TKB_ARGS a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st
-  if (M <= 16) return launch_few<16, GATED, T>(TKB_ARGS);
-  if (M <= 32) return launch_few<32, GATED, T>(TKB_ARGS);
-  if (M <= 64) return launch_few<64, GATED, T>(TKB_ARGS);
-  if (M <= 128) return launch_few<128, GATED, T>(TKB_ARGS);
-  const long long few_tiles = (long long)((N + BC - 1) / BC) * ((M + 255) / 256);
-  if (2 * few_tiles <= sm_count()) return launch_few<256, GATED, T>(TKB_ARGS);
+#define TKB_ARGS_FEW a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, p.parts, p.per, weights_ready, status, st
+  const Plan p = plan(M, N, K);
+  switch (p.tokens) {
+    case 16: return launch_few<16, GATED, T>(TKB_ARGS_FEW);
+    case 32: return launch_few<32, GATED, T>(TKB_ARGS_FEW);
+    case 64: return launch_few<64, GATED, T>(TKB_ARGS_FEW);
+    case 128: return launch_few<128, GATED, T>(TKB_ARGS_FEW);
+  }
   if (N >= 256) return launch_many<256, GATED, T>(TKB_ARGS);
   return launch_many<128, GATED, T>(TKB_ARGS);
 #undef TKB_ARGS
