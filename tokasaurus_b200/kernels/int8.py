@@ -56,10 +56,6 @@ def _stride0(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _code_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
-
-
 def _code_rows(rows: int, k: int, device) -> torch.Tensor:
     """Room for rows of codes, each on a 16-byte boundary."""
     return torch.empty((rows, (k + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :k]
@@ -70,20 +66,26 @@ def _check_rows(what: str, x: torch.Tensor) -> None:
         raise KernelError(f"{what}: rows of numbers that lie together")
 
 
-def _check_codes(what: str, t: torch.Tensor, scale: torch.Tensor) -> None:
-    if not (t.dtype == torch.int8 and t.dim() == 2 and 1 <= t.shape[1] <= MAX_K):
+def _check_codes(what: str, t: torch.Tensor, scale: torch.Tensor) -> tuple[int, int, int]:
+    """Rows, codes a row, and the row stride of codes that the products take."""
+    shape = t.shape
+    if not (t.dtype == torch.int8 and len(shape) == 2 and 1 <= shape[1] <= MAX_K):
         raise KernelError(f"{what}: int8 rows of 1 to {MAX_K} codes (the sum of a longer row's products need not fit 32 bits)")
-    n, k = t.shape
-    if not ((t.stride(1) == 1 or k == 1) and (n <= 1 or t.stride(0) % 16 == 0) and t.data_ptr() % 16 == 0):
+    n, k = shape
+    stride, one = t.stride()
+    if n <= 1:
+        stride = (k + 15) // 16 * 16
+    if not ((one == 1 or k == 1) and stride % 16 == 0 and t.data_ptr() % 16 == 0):
         raise KernelError(f"{what}: rows of codes lie on 16-byte boundaries (quantise_rows and lay_out_codes leave them so)")
     if not (scale.dtype == torch.float32 and scale.numel() == n and scale.is_contiguous()):
         raise KernelError(f"{what}: a float32 scale a row of codes")
+    return n, k, stride
 
 
-def _check_product(what: str, k: int, w: torch.Tensor, gated: bool) -> None:
-    if w.shape[1] != k or w.shape[0] < 1:
+def _check_product(what: str, k: int, w_rows: int, w_k: int, gated: bool) -> None:
+    if w_k != k or w_rows < 1:
         raise KernelError(f"{what}: as many numbers in a row of tokens as of weights [N, K]")
-    if gated and w.shape[0] % 16:
+    if gated and w_rows % 16:
         raise KernelError(f"{what}: gated weights come in groups of 16 rows")
 
 
@@ -108,15 +110,13 @@ def product_int8(codes: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_sc
     silu(gate) * up [M, N / 2]."""
     what = "product_int8"
     _need_cuda(codes, scale, w, w_scale, status)
-    _check_codes(what, codes, scale)
-    _check_codes(what, w, w_scale)
-    M, K = codes.shape
-    N = w.shape[0]
-    _check_product(what, K, w, gated)
+    M, K, stride = _check_codes(what, codes, scale)
+    N, w_k, w_stride = _check_codes(what, w, w_scale)
+    _check_product(what, K, N, w_k, gated)
     cols = N // 2 if gated else N
     out = torch.empty((M, cols), dtype=out_dtype, device=codes.device)
     _check(_entry("int8_product.cu", "tkb_int8_product")(
-        codes.data_ptr(), _code_stride(codes), scale.data_ptr(), w.data_ptr(), _code_stride(w), w_scale.data_ptr(), out.data_ptr(), cols,
+        codes.data_ptr(), stride, scale.data_ptr(), w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols,
         _is_f32(out_dtype), M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
     return out
 
@@ -128,19 +128,18 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status:
     what = "linear_int8"
     _need_cuda(x, w, w_scale, status)
     _check_rows(what, x)
-    _check_codes(what, w, w_scale)
+    N, w_k, w_stride = _check_codes(what, w, w_scale)
     M, K = x.shape
-    N = w.shape[0]
-    _check_product(what, K, w, gated)
+    _check_product(what, K, N, w_k, gated)
     x_dtype = x.dtype
     out_dtype = out_dtype or x_dtype
     x_f32, f32 = _is_f32(x_dtype), _is_f32(out_dtype)
     cols = N // 2 if gated else N
-    device = x.device
-    out = torch.empty((M, cols), dtype=out_dtype, device=device)
-    scratch = torch.empty(((M * 4 + 15) // 16 * 16 + M * ((K + 15) // 16 * 16),), dtype=torch.int8, device=device)
+    # (new_empty without a type costs a quarter less on the host than torch.empty)
+    out = x.new_empty((M, cols)) if out_dtype == x_dtype else x.new_empty((M, cols), dtype=out_dtype)
+    scratch = w.new_empty(((M * 4 + 15) // 16 * 16 + M * ((K + 15) // 16 * 16),))
     _check(_entry("int8_product.cu", "tkb_linear_int8")(
-        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), _code_stride(w), w_scale.data_ptr(), out.data_ptr(), cols, f32, scratch.data_ptr(),
+        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols, f32, scratch.data_ptr(),
         M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
     ops.LAUNCHES += 1  # two kernels
     return out
@@ -284,8 +283,7 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
         if singles == 0:
             return
         which, tokens, requests = 1, singles, singles
-    scratch = torch.empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group),),
-                          dtype=torch.uint8, device=q.device)
+    scratch = kcache.new_empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group),))
     _check(_entry("attention_kv8.cu", "tkb_attn_kv8", head_dim)(
         *common, scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window, pool, which,
         status.data_ptr(), _stream()), what)
