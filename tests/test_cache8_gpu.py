@@ -382,3 +382,96 @@ def test_refusals():
         a.update(bad)
         with pytest.raises(KernelError):
             int8.read_kv8(**a)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("ps", [5, 64, 256])
+def test_write_rotates_into_pages_of_other_sizes(ps, dtype):
+    """Portions that fill parts of pages, whole pages and several, with the numbers rotated: codes are those of the numbers that the
+    rotation with pages of 16 gives."""
+    lengths = [(300, 333), (1, 70), (64, 64), (7, 130)]
+    st, ref = Step(lengths, 4, 2, 64, ps, dtype, seed=9), Step(lengths, 4, 2, 64, 16, dtype, seed=9)
+    ref.rows = st.rows.clone()
+    inv = (10000.0 ** (-torch.arange(32) / 32)).float().to(DEV)
+    from tokasaurus_b200.kernels import int8, ops
+
+    k = torch.zeros(st.pool, 2, ps, 64, device=DEV, dtype=dtype)
+    v = torch.zeros_like(k)
+    plain = st.rows.clone()
+    ops.rope_kv_write(plain, i32(st.pos), i32(st.seq), i32(st.first), i32(st.ids), inv, k, v, 4, 2, 64, 64, ps, True, st.status)
+    st.write(inv, 64)
+    ref.write(inv, 64)
+    assert torch.equal(st.rows, ref.rows)  # q does not know of pages
+    got = int8.read_kv8(st.kc, st.vc, st.ks, st.vs, i32(np.arange(st.pool)), st.status)
+    for s, (q, kv) in enumerate(lengths):
+        for p in range(kv - q, kv):
+            page, slot = st.ids[st.first[s] + p // ps], p % ps
+            for g, want, sc in ((got[0], k, st.ks), (got[1], v, st.vs)):
+                w = want[page, :, slot].double()
+                # half a code, and half a code again if the block's scale grew later; the rotation's rounding
+                grew = 1.0 if (kv - q) % ps else 0.5
+                assert ((g[page, :, slot].double() - w).abs() <= sc[page].double()[:, None] * (grew + 0.001) + w.abs() * (2.0**-8 if dtype == BF else 2.0**-20)).all()
+    assert int(st.status) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("q_stride", [8 * 64 + 1, 8 * 64 + 4])
+def test_attention_of_rows_on_any_boundary(q_stride, dtype):
+    st = Step([(1, 700), (70, 150), (1, 3)], 8, 2, 64, 16, dtype, q_stride=q_stride)
+    want = st.check_attention()
+    q = st.q
+    st.q = q.contiguous()
+    assert torch.equal(st.attend(), want)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_in_a_graph_with_other_lengths(hd):
+    """A launch that is replayed: the requests' lengths change in place, up to what the launch was sized for; idle rows bring none."""
+    from tokasaurus_b200.kernels import int8
+
+    n = 6
+    st = Step([(1, 4000)] * n, 8, 2, hd, 16, BF, seed=2)
+    q_len, kv_len = i32([1] * n), i32([4000] * n)
+    out = torch.empty(n, 8 * hd, dtype=BF, device=DEV)
+
+    def call():
+        int8.attn_kv8(st.q, out, st.kc, st.vc, st.ks, st.vs, i32_starts, q_len, kv_len, first, ids, 8, 2, hd, 16, hd**-0.5, None, st.status,
+                      max_q_len=1, max_kv_len=4000, single_tokens=n)
+
+    i32_starts, first, ids = i32(st.starts[:-1]), i32(st.first), i32(st.ids)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+        call()  # (two launches of one step share the graph's memory)
+    for lengths in ([4000] * n, [1, 4000, 17, 600, 2000, 3], [5] * n, [3999, 0, 0, 0, 0, 0], [4000] * n):
+        q_len.copy_(i32([int(kv > 0) for kv in lengths]))
+        kv_len.copy_(i32(lengths))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        live = [s for s in range(n) if lengths[s] > 0]
+        alone = Step([(1, max(kv, 1)) for kv in lengths], 8, 2, hd, 16, BF, seed=2)
+        alone.kc, alone.vc, alone.ks, alone.vs, alone.pool = st.kc, st.vc, st.ks, st.vs, st.pool
+        alone.q = st.q
+        alone.ids = [st.ids[st.first[s] + i] for s in range(n) for i in range(-(-max(lengths[s], 1) // 16))]
+        want = alone.check_attention()
+        # the same keys in other shares: float32 sums in another order, and the result's rounding
+        assert ((out[live].double() - want[live].double()).abs() <= want[live].double().abs() * 2.0**-7 + 2.0**-10 * 127 * st.vs.max().double()).all()
+    assert int(st.status) == 0
+
+
+def test_attention_and_write_on_another_stream():
+    st, ref = (Step([(1, 2000)] * 4 + [(50, 90)], 8, 2, 64, 16, BF, seed=4) for _ in range(2))
+    ref.write()
+    want = ref.attend()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        st.write()
+        got = st.attend()
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(st.kc, ref.kc) and torch.equal(st.vs, ref.vs)

@@ -202,3 +202,73 @@ def test_refusals():
                                           torch.zeros(1, 132112, dtype=torch.int8, device=DEV), t[:1].contiguous(), st)):
         with pytest.raises(KernelError):
             bad()
+
+
+@pytest.mark.parametrize("m,k,n,gated", [(3, 14336, 256, False), (20, 8192, 130, False), (40, 4096, 128, True), (100, 14336, 512, False), (129, 2048, 640, True),
+                                         (130, 8192, 2048, False), (200, 4096, 1040, True), (256, 4096, 6144, False), (300, 8192, 96, False), (700, 1000, 272, True)])
+def test_tiles_of_tokens_and_parts_of_k(m, k, n, gated):
+    """Sizes at which tokens come in one tile or several and K in one part or up to eight: each result as its rows alone give it, and
+    some of them against the definition."""
+    from tokasaurus_b200.kernels import int8
+
+    x = rows(m, k, BF, seed=m + n)
+    w, t = codes(n, k, seed=k)
+    t = t / k**0.5
+    st = status()
+    y = int8.linear_int8(x, w, t, st, gated=gated, out_dtype=F32)
+    c, s = plain_quantise(x)
+    z = (c.to(DEV).double() @ w.double().t()) * s.to(DEV).double()[:, None] * t.double()
+    if gated:
+        z = z.view(m, n // 16, 2, 8)
+        g, u = z[:, :, 0].reshape(m, -1), z[:, :, 1].reshape(m, -1)
+        want = g * torch.sigmoid(g) * u
+        bound = want.abs() * (6 * g.abs() + 24) * U32 + 2.0**-120
+        bound = torch.where(g.abs() < 80, bound, 1e-30 + want.abs() * 12 * U32)
+    else:
+        want = z
+        bound = want.abs() * 3.01 * U32 + 2.0**-126
+    assert ((y.double() - want).abs() <= bound).all() and int(st) == 0
+    for lo, hi in ((0, 1), (m // 2, m // 2 + 9), (max(0, m - 70), m)):
+        assert torch.equal(int8.linear_int8(x[lo:hi], w, t, st, gated=gated, out_dtype=F32), y[lo:hi])
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_weights_made_right_before(m):
+    """Nothing stands between the kernel that makes the weights' codes and the product that reads them."""
+    from tokasaurus_b200.kernels import int8
+
+    st = status()
+    xs = [rows(m, 1024, BF, seed=i) for i in range(8)]
+    ws = [rows(768, 1024, BF, seed=20 + i) for i in range(8)]
+    made = [int8.quantise_rows(w) for w in ws]
+    torch.cuda.synchronize()
+    want = [int8.linear_int8(x, *cw, st) for x, cw in zip(xs, made)]
+    torch.cuda.synchronize()
+    got = []
+    for x, w in zip(xs, ws):
+        got.append((int8.linear_int8(x, *int8.quantise_rows(w), st), int8.product_int8(*int8.quantise_rows(x), *int8.quantise_rows(w), st)))
+    for a, (b, c) in zip(want, got):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert int(st) == 0
+
+
+def test_products_in_a_graph():
+    """Replays of a captured step with other tokens in place."""
+    from tokasaurus_b200.kernels import int8
+
+    st = status()
+    x, (w, t) = rows(9, 2048, BF), codes(512, 2048)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        int8.linear_int8(x, w, t, st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = int8.linear_int8(x, w, t, st)
+        z = int8.linear_int8(y, w[:, :512], t, st)
+    for seed in range(3):
+        x.copy_(rows(9, 2048, BF, seed=100 + seed))
+        graph.replay()
+        a = int8.linear_int8(x, w, t, st)
+        assert torch.equal(y, a) and torch.equal(z, int8.linear_int8(a, w[:, :512], t, st))
+    assert int(st) == 0
