@@ -617,14 +617,204 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
 #undef TKB_ARGS
 }
 
+// ------------------------------------------------------------------------------------------------ up to 8 tokens, in one launch
+// A block an SM brings all tokens to codes in shared memory (each block for itself: K numbers of a few tokens are little beside the
+// weights) while its first weights are on their way to registers, where they stay: a warp takes 16 channels and a slice of K,
+//     mma.sync 16 channels x 8 tokens x 32 in 8-bit integers,
+// a lane 16 codes of two channels a load, which serve two instructions (the tokens' codes are read in the same order of K, so that
+// neither side is rearranged).  Slices are added up in shared memory.  Gate and up rows of a group of 16 meet in one warp.
+constexpr int ROWS_WARPS = 16, ROWS_TOKENS = 8, ROWS_STEPS = 4;  // steps of 64 codes a turn
+constexpr int ROWS_NUMBERS = 32768;                              // of all tokens, at most
+constexpr long long ROWS_WEIGHTS = 1ll << 25;
+
+__device__ __forceinline__ uint4 load_weights(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <bool GATED, typename X, typename T>
+__global__ void __launch_bounds__(ROWS_WARPS * 32, 1)
+product_rows_kernel(const X* __restrict__ x, long long ldx, const int8_t* __restrict__ w, long long ldw, const float* __restrict__ w_scale,
+                    T* __restrict__ out, long long ldo, int M, int N, int K, int slices_log2, int stride) {
+  constexpr int SUM_STRIDE = 16 * ROWS_TOKENS + 8;
+  extern __shared__ __align__(16) unsigned char codes[];  // M rows, `stride` bytes apart
+  __shared__ int sums[2][ROWS_WARPS][SUM_STRIDE];         // [token][channel]
+  __shared__ unsigned s_top[ROWS_TOKENS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int slices = 1 << slices_log2, per_round = ROWS_WARPS >> slices_log2;  // channel groups of 16 a block and round
+  const int groups = (N + 15) >> 4, rounds = (groups + per_round * gridDim.x - 1) / (per_round * gridDim.x);
+  const int steps = (K + 63) >> 6, slice = warp & (slices - 1), slot = warp >> slices_log2;
+  const int per = (steps + slices - 1) >> slices_log2, s_begin = slice * per, s_end = min(steps, s_begin + per);
+  const int turns = (per + ROWS_STEPS - 1) / ROWS_STEPS;
+  auto group_of = [&](int round) { return (round * per_round + slot) * (int)gridDim.x + (int)blockIdx.x; };
+  auto row_of = [&](int round, int r) { return w + (long long)min(group_of(round) * 16 + r, N - 1) * ldw; };
+  trigger_dependents();
+  if (threadIdx.x < ROWS_TOKENS) s_top[threadIdx.x] = 0;
+  {
+    // the second-level cache may fetch the first weights before the kernel ahead is over (they are read only behind it)
+    const int at = min(s_begin * 64 + c * 128, K - 16);
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row_of(0, g) + at));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row_of(0, g + 8) + at));
+  }
+  grid_dependency_wait();
+
+  uint4 a[2][ROWS_STEPS][2];
+  const int8_t *row0, *row1;
+  auto load = [&](int round, int turn, uint4 (&v)[ROWS_STEPS][2]) {
+    if (turn == 0) row0 = row_of(round, g), row1 = row_of(round, g + 8);
+#pragma unroll
+    for (int u = 0; u < ROWS_STEPS; u++) {
+      const int at = min((s_begin + turn * ROWS_STEPS + u) * 64 + c * 16, K - 16);  // (codes of tokens behind K are zeros)
+      v[u][0] = load_weights(row0 + at);
+      v[u][1] = load_weights(row1 + at);
+    }
+  };
+  load(0, 0, a[0]);
+
+  // ---------------- tokens to codes: a power of two of warps a token
+  {
+    int log2_m = 0;
+    while ((1 << log2_m) < M) log2_m++;
+    const int warps = ROWS_WARPS >> log2_m, m = warp / warps, first = (warp % warps) * 32 + lane, step = warps * 32, eights = K >> 3;
+    constexpr int HELD = sizeof(X) == 2 ? 8 : 4;
+    Eight<X, true> mine[HELD];
+    const X* row = x + (long long)min(m, M - 1) * ldx;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) mine[i].load(row + 8 * min(first + i * step, eights - 1));
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) top = max(top, magnitude(mine[i].at(j)));
+    for (int e = first + HELD * step; e < eights; e += step) {
+      Eight<X, true> v;
+      v.load(row + 8 * e);
+#pragma unroll
+      for (int j = 0; j < 8; j++) top = max(top, magnitude(v.at(j)));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    __syncthreads();  // (s_top is zero)
+    if (lane == 0) atomicMax(&s_top[m], top);
+    __syncthreads();
+    if (m < M) {
+      top = s_top[m];
+      const bool finite = top < NOT_FINITE;
+      const float s = finite ? __uint_as_float(top) * ONE_127TH : NAN;
+      const float inv = 1.f / s;
+      const bool some = finite && s > 0.f;
+      auto put = [&](int e, const Eight<X, true>& v) {
+        *reinterpret_cast<uint2*>(codes + m * stride + 8 * e) =
+            some ? make_uint2(four_codes(make_float4(v.at(0), v.at(1), v.at(2), v.at(3)), s, inv),
+                              four_codes(make_float4(v.at(4), v.at(5), v.at(6), v.at(7)), s, inv))
+                 : make_uint2(0, 0);
+      };
+#pragma unroll
+      for (int i = 0; i < HELD; i++)
+        if (first + i * step < eights) put(first + i * step, mine[i]);
+      for (int e = first + HELD * step; e < eights; e += step) {
+        Eight<X, true> v;
+        v.load(row + 8 * e);
+        put(e, v);
+      }
+      for (int e = eights + first; e < steps * 8; e += step) *reinterpret_cast<uint2*>(codes + m * stride + 8 * e) = make_uint2(0, 0);
+    }
+    __syncthreads();
+  }
+  auto scale_of = [&](int m) {
+    const unsigned top = s_top[m];
+    return top < NOT_FINITE ? __uint_as_float(top) * ONE_127TH : NAN;
+  };
+  const unsigned char* b_row = codes + min(g, M - 1) * stride + c * 16;
+
+  // ---------------- products
+  int d[4] = {};
+  auto multiply = [&](int turn, const uint4 (&v)[ROWS_STEPS][2]) {
+#pragma unroll
+    for (int u = 0; u < ROWS_STEPS; u++) {
+      const int st = s_begin + turn * ROWS_STEPS + u;
+      if (st < s_end) {
+        const uint4 b = *reinterpret_cast<const uint4*>(b_row + st * 64);
+        mma8(d, v[u][0].x, v[u][1].x, v[u][0].y, v[u][1].y, b.x, b.y);
+        mma8(d, v[u][0].z, v[u][1].z, v[u][0].w, v[u][1].w, b.z, b.w);
+      }
+    }
+  };
+  auto finish_round = [&](int round) {
+    int* mine = sums[round & 1][warp];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      mine[(2 * c + (e & 1)) * 16 + g + 8 * (e >> 1)] = d[e];
+      d[e] = 0;
+    }
+    __syncthreads();
+    constexpr int OUTS = GATED ? 8 : 16;  // a group's results of a token
+    for (int i = threadIdx.x; i < per_round * M * OUTS; i += ROWS_WARPS * 32) {
+      const int f = i % OUTS, m = i / OUTS % M, at = i / OUTS / M;
+      const int group = (round * per_round + at) * (int)gridDim.x + (int)blockIdx.x, n = group * 16 + f;
+      int sum = 0, up = 0;
+      for (int p = 0; p < slices; p++) {
+        const int* from = sums[round & 1][(at << slices_log2) + p] + m * 16 + f;
+        sum += from[0];
+        if (GATED) up += from[8];
+      }
+      if (n + (GATED ? 8 : 0) < N) {
+        const float s = scale_of(m);
+        float y = value_of((uint32_t)sum, s * w_scale[n]);
+        if (GATED) y = silu_mul_fast(y, value_of((uint32_t)up, s * w_scale[n + 8]));
+        out[(long long)m * ldo + (GATED ? group * 8 + f : n)] = from_float<T>(y);
+      }
+    }
+  };
+  int round = 0, turn = 0;
+  auto step_on = [&](const uint4 (&now)[ROWS_STEPS][2], uint4 (&then)[ROWS_STEPS][2]) {
+    const int next_turn = turn + 1 == turns ? 0 : turn + 1, next_round = next_turn == 0 ? round + 1 : round;
+    if (next_round < rounds) load(next_round, next_turn, then);
+    multiply(turn, now);
+    if (next_turn == 0) finish_round(round);
+    turn = next_turn, round = next_round;
+  };
+  while (round < rounds) {
+    step_on(a[0], a[1]);
+    if (round < rounds) step_on(a[1], a[0]);
+  }
+}
+
+// Rows of codes in shared memory: an odd number of 64 bytes apart, so that two tokens' reads meet no bank twice.
+int rows_stride(int K) { return ((K + 63) / 64 | 1) * 64; }
+bool takes_rows(const void* x, long long ldx, int x_f32, int M, int N, int K) {
+  const int bytes = x_f32 ? 4 : 2;
+  return M <= ROWS_TOKENS && K % 16 == 0 && (long long)M * K <= ROWS_NUMBERS && (long long)N * K <= ROWS_WEIGHTS && (((uintptr_t)x) & 15) == 0 &&
+         (M == 1 || ldx * bytes % 16 == 0);
+}
+
+template <bool GATED, typename X, typename T>
+int launch_rows(const void* x, long long ldx, const void* w, long long ldw, const float* w_scale, void* out, long long ldo, int M, int N, int K, cudaStream_t st) {
+  static SharedMemoryRequest ask;
+  int rc = ask({{(const void*)product_rows_kernel<GATED, X, T>, ROWS_NUMBERS + ROWS_TOKENS * 128}});
+  if (rc) return rc;
+  const int groups = (N + 15) / 16, blocks = groups < sm_count() ? groups : sm_count();
+  int log2_slices = 4;
+  while (log2_slices > 0 && (long long)(ROWS_WARPS >> log2_slices) * blocks < groups) log2_slices--;
+  const int stride = rows_stride(K);
+  return launch_pdl(product_rows_kernel<GATED, X, T>, dim3(blocks), dim3(ROWS_WARPS * 32), (size_t)M * stride, st, (const X*)x, ldx, (const int8_t*)w, ldw,
+                    w_scale, (T*)out, ldo, M, N, K, log2_slices, stride);
+}
+int check(const void* w, long long ldw, int K, int N, int gated) {
+  return K <= 0 || K > 132103 || (gated && (N & 15)) || (ldw & 15) || (((uintptr_t)w) & 15) ? -2 : 0;
+}
+
 // a, w: codes whose rows start on 16-byte boundaries (row strides lda, ldw in bytes).  weights_ready: the kernel ahead in the
 // stream is the one that makes the tokens' codes, so that no kernel that may still be running writes w.
 int product_any(const void* a, long long lda, const float* a_scale, const void* w, long long ldw, const float* w_scale, void* out,
                 long long ldo, int f32, int M, int N, int K, int gated, int weights_ready, int* status, cudaStream_t st) {
   if (M <= 0 || N <= 0) return 0;
-  if (K <= 0 || K > 132103 || (gated && (N & 15)) || (lda & 15) || (ldw & 15) || (((uintptr_t)a) & 15) || (((uintptr_t)w) & 15)) return -2;
-  int rc = get_encode();
-  if (rc) return rc;
+  int rc = (lda & 15) || (((uintptr_t)a) & 15) ? -2 : check(w, ldw, K, N, gated);
+  if (rc || (rc = get_encode())) return rc;
   if (gated)
     return f32 ? product<true, float>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st)
                : product<true, bf16>(a, lda, a_scale, w, ldw, w_scale, out, ldo, M, N, K, weights_ready, status, st);
@@ -642,14 +832,31 @@ TKB_EXPORT int tkb_quantise_rows(const void* x, long long ldx, int f32, void* co
   return f32 ? quantise<float>(x, ldx, codes, ldc, (float*)scale, M, K, st) : quantise<bf16>(x, ldx, codes, ldc, (float*)scale, M, K, st);
 }
 
-// Both in one call: scratch has room for M float32 (padded to 16 bytes), then M rows of K codes padded to 16 bytes each.
+// Bytes of scratch that tkb_linear_int8 wants with the same arguments: M float32 (padded to 16 bytes), then M rows of K codes padded
+// to 16 bytes each, or none where the product makes the codes itself.
+TKB_EXPORT long long tkb_linear_int8_scratch(const void* x, long long ldx, int x_f32, int M, int N, int K) {
+  return M <= 0 || K <= 0 || takes_rows(x, ldx, x_f32, M, N, K) ? 0 : ((long long)M * 4 + 15) / 16 * 16 + M * (((long long)K + 15) / 16 * 16);
+}
+
+// Both in one call.
 TKB_EXPORT int tkb_linear_int8(const void* x, long long ldx, int x_f32, const void* w, long long ldw, const float* w_scale, void* out,
                                long long ldo, int f32, void* scratch, int M, int N, int K, int gated, int* status, void* st) {
   if (M <= 0 || N <= 0) return 0;
+  int rc = check(w, ldw, K, N, gated);
+  if (rc) return rc;
+  if (takes_rows(x, ldx, x_f32, M, N, K)) {
+#define TKB_ARGS x, ldx, w, ldw, w_scale, out, ldo, M, N, K, (cudaStream_t)st
+    if (gated)
+      return x_f32 ? f32 ? launch_rows<true, float, float>(TKB_ARGS) : launch_rows<true, float, bf16>(TKB_ARGS)
+                   : f32 ? launch_rows<true, bf16, float>(TKB_ARGS) : launch_rows<true, bf16, bf16>(TKB_ARGS);
+    return x_f32 ? f32 ? launch_rows<false, float, float>(TKB_ARGS) : launch_rows<false, float, bf16>(TKB_ARGS)
+                 : f32 ? launch_rows<false, bf16, float>(TKB_ARGS) : launch_rows<false, bf16, bf16>(TKB_ARGS);
+#undef TKB_ARGS
+  }
   float* scale = (float*)scratch;
   char* codes = (char*)scratch + ((size_t)M * 4 + 15) / 16 * 16;
   const long long ldc = ((long long)K + 15) / 16 * 16;
-  const int rc = tkb_quantise_rows(x, ldx, x_f32, codes, ldc, scale, M, K, st);
+  rc = tkb_quantise_rows(x, ldx, x_f32, codes, ldc, scale, M, K, st);
   return rc ? rc : product_any(codes, ldc, scale, w, ldw, w_scale, out, ldo, f32, M, N, K, gated, 1, status, (cudaStream_t)st);
 }
 

@@ -30,6 +30,7 @@ _ARGS = {
     "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _I, _P, _P),
     "tkb_attn_kv8_tc": (_P, _L, _P, _L, _I) + (_P,) * 9 + (_I,) * 6 + (_F, _I, _I, _P, _P),
     "tkb_attn_kv8_scratch": (_I,) * 6,
+    "tkb_linear_int8_scratch": (_P, _L, _I, _I, _I, _I),
     "tkb_linear_int8": (_P, _L, _I, _P, _L, _P, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P),
 }
 _functions: dict = {}
@@ -137,11 +138,13 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status:
     cols = N // 2 if gated else N
     # (new_empty without a type costs a quarter less on the host than torch.empty)
     out = x.new_empty((M, cols)) if out_dtype == x_dtype else x.new_empty((M, cols), dtype=out_dtype)
-    scratch = w.new_empty(((M * 4 + 15) // 16 * 16 + M * ((K + 15) // 16 * 16),))
+    need = _entry("int8_product.cu", "tkb_linear_int8_scratch")(x.data_ptr(), x.stride(0), x_f32, M, N, K)
+    scratch = w.new_empty((need,)) if need else None
     _check(_entry("int8_product.cu", "tkb_linear_int8")(
-        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols, f32, scratch.data_ptr(),
-        M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
-    ops.LAUNCHES += 1  # two kernels
+        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols, f32,
+        scratch.data_ptr() if need else None, M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
+    if need:
+        ops.LAUNCHES += 1  # two kernels
     return out
 
 
