@@ -624,7 +624,7 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
 // a lane 16 codes of two channels a load, which serve two instructions (the tokens' codes are read in the same order of K, so that
 // neither side is rearranged).  Slices are added up in shared memory.  Gate and up rows of a group of 16 meet in one warp.
 constexpr int ROWS_WARPS = 16, ROWS_TOKENS = 8, ROWS_STEPS = 4;  // steps of 64 codes a turn
-constexpr int ROWS_NUMBERS = 32768;                              // of all tokens, at most
+constexpr int ROWS_NUMBERS = 8192;                              // of all tokens, at most
 constexpr long long ROWS_WEIGHTS = 1ll << 25;
 
 __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
