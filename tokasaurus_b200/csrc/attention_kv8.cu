@@ -47,6 +47,7 @@ constexpr bool SWIZZLES = HD == 64 || HD == 128;
 constexpr int WINDOW = 64;           // pages that are looked up together; a tile has no more
 constexpr float SLACK = 8.f;
 constexpr int WHOLE_KEYS = 512;       // up to so many keys a request's items are not cut
+constexpr int OWN_TILES = 4;          // tiles by which shares of one item may be longer than even ones
 constexpr float LOWEST = -1e30f;  // a reference before the first key
 
 __host__ __device__ constexpr int max_nt() { return HD <= 128 ? 2 : 1; }
@@ -160,7 +161,7 @@ constexpr int SINGLE = 1, PORTION = 2;  // `which`
 
 // One request's part of the work.
 struct Request {
-  int s, q_len, kv_len, q_start, table, col_tiles, k0, tiles;
+  int s, q_len, kv_len, q_start, table, col_tiles, k0, tiles, row;  // row: tiles and what fills them up to whole shares
   template <typename L> __device__ __forceinline__ bool load(const Args& a, int s_) {
     constexpr int BKV = L::BKV, cols = L::COLS;
     s = s_;
@@ -172,16 +173,16 @@ struct Request {
     col_tiles = (q_len * a.out.group + cols - 1) / cols;
     const int first = a.window > 0 ? max(0, kv_len - q_len - a.window + 1) : 0;
     k0 = first & ~(BKV - 1);
-    tiles = max(1, (kv_len - k0 + BKV - 1) / BKV);
+    row = tiles = max(1, (kv_len - k0 + BKV - 1) / BKV);
     return true;
   }
-  __device__ __forceinline__ int work() const { return col_tiles * tiles; }
+  __device__ __forceinline__ void fill_up(int each) { row = (tiles + each - 1) / each * each; }
+  __device__ __forceinline__ int work() const { return col_tiles * row; }
 };
 
-// The row of all tiles in `n` even shares: the first `rest` of them hold one tile more.
+// The row of all tiles in shares of `each`, the first `rest` of them with one tile more.
 struct Shares {
   int each, rest;
-  __device__ __forceinline__ Shares(int total, int n) : each(total / n), rest(total % n) {}
   __device__ __forceinline__ int start(int b) const { return b * each + min(b, rest); }
   // the share that holds tile x
   __device__ __forceinline__ int of(int x) const {
@@ -202,11 +203,12 @@ struct Walk {
   int tile_end;          // one past the last one of this item in the share
   int at, end;           // in the row of all tiles
   bool live, opens;      // opens: the share starts with this item
+  bool one;              // the share holds one item
   __device__ __forceinline__ void clip() { tile_end = end - at < r.tiles - tile ? tile + (end - at) : r.tiles; }
   template <typename L> __device__ __forceinline__ void next_item(const Args& a) {
     at += tile_end - tile;
     opens = false;
-    live = at < end;
+    live = !one && at < end;
     if (!live) return;
     tile = 0;
     if (++ct == r.col_tiles) {
@@ -332,7 +334,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
   __shared__ float s_qs[COLS], s_M[WARPS][COLS], s_m[WARPS][COLS], s_l[WARPS][COLS];
-  __shared__ int s_scan[THREADS / 32], s_offset, s_seq;
+  __shared__ int s_scan[2][THREADS / 32], s_offset, s_seq;
   __shared__ Request s_first;
   __shared__ CutItem s_cut[2];  // the item that the share starts with, and one that it ends with, if they are cut (n: their parts)
   __shared__ uint32_t s_there[STAGES][BKV / 32];  // pages (keys) of a tile that the request still holds, a bit each
@@ -362,31 +364,54 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   // ---------------- this block's share of the row of all tiles
   const int per = (a.n_seqs + THREADS - 1) / THREADS;
   const int lo = min(a.n_seqs, (int)threadIdx.x * per), hi = min(a.n_seqs, lo + per);
-  int mine = 0;
   Request rq;
+  int mine = 0, items = 0;  // tiles and column tiles
   for (int s = lo; s < hi; s++)
-    if (rq.load<L>(a, s)) mine += rq.work();
-  int before = mine;
+    if (rq.load<L>(a, s)) mine += rq.work(), items += rq.col_tiles;
+  int before, total;
+  auto scan = [&]() {  // of `mine`: what stands before this thread's, and all
+    before = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
-  }
-  if (lane == 31) s_scan[warp] = before;
-  __syncthreads();
-  int total = 0;
-  before -= mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    if (lane == 31) s_scan[0][warp] = before;
+    const int warp_items = __reduce_add_sync(0xffffffffu, items);
+    if (lane == 0) s_scan[1][warp] = warp_items;
+    __syncthreads();
+    total = 0, items = 0;
+    before -= mine;
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; i++) {
-    if (i < warp) before += s_scan[i];
-    total += s_scan[i];
+    for (int i = 0; i < THREADS / 32; i++) {
+      if (i < warp) before += s_scan[0][i];
+      total += s_scan[0][i];
+      items += s_scan[1][i];
+    }
+  };
+  scan();
+  Shares shares{total / (int)gridDim.x, total % (int)gridDim.x};
+  // Even shares hold parts of two items here and there: twice the way from queries to results, and two joins.  Where shares that start
+  // with their items, as many tiles each, are little longer, those are taken.
+  const int even = shares.each + (shares.rest > 0), own = items < (int)gridDim.x ? (total + gridDim.x - items - 1) / (gridDim.x - items) : 0x7fffffff;
+  const bool one = !a.whole && own - OWN_TILES <= even;
+  if (one) {
+    shares = {own, 0};
+    mine = 0;
+    for (int s = lo; s < hi; s++)
+      if (rq.load<L>(a, s)) {
+        rq.fill_up(own);
+        mine += rq.work();
+      }
+    __syncthreads();  // (s_scan has been read)
+    scan();
   }
-  const Shares shares(total, gridDim.x);
   const int start = shares.start(blockIdx.x), end = shares.start(blockIdx.x + 1);
   if (start >= before && start < before + mine) {
     int at = before;
     for (int s = lo; s < hi; s++)
       if (rq.load<L>(a, s)) {
+        if (one) rq.fill_up(own);
         if (start < at + rq.work()) {
           s_seq = s;
           s_offset = start - at;
@@ -401,8 +426,9 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   w.live = s_seq >= 0 && start < end;
   if (w.live) {
     w.r = s_first;
-    w.ct = w.r.col_tiles == 1 ? 0 : s_offset / w.r.tiles;
-    w.tile = s_offset - w.ct * w.r.tiles;
+    w.ct = w.r.col_tiles == 1 ? 0 : s_offset / w.r.row;
+    w.tile = s_offset - w.ct * w.r.row;
+    w.one = one;
     w.at = start;
     w.end = end;
     w.opens = true;
