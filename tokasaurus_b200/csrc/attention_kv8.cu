@@ -119,7 +119,7 @@ __device__ __forceinline__ uint32_t rest_half(uint32_t h, float lo, float hi) {
 __device__ __forceinline__ int key_of_row(int r) { return HD == 64 ? r ^ ((r >> 1) & 1) : (r & 8) | ((r & 1) ? (r & 6) ^ 5 : r & 6); }
 // Where byte `at` of key k lies in the ring.  A 128-byte row is one key's of 128 codes or two keys' of 64; its 16-byte chunks are
 // exclusive-or the row's number, as TMA leaves them.
-__device__ __forceinline__ int place(int k, int at, bool swizzled) {
+[[maybe_unused]] __device__ __forceinline__ int place(int k, int at, bool swizzled) {
   const int x = k * HD + at;
   return SWIZZLES && swizzled ? x ^ ((HD == 128 ? k & 7 : (k >> 1) & 7) << 4) : x;
 }
@@ -266,21 +266,42 @@ __device__ __forceinline__ bool arrive(unsigned long long* word, int n) {
 }
 
 // An item's `n` parts (the first stands at `first`, part i of the others at rest + 2 i parts) into its result, by 128 threads: the
-// columns' references and sums by every warp, then 32 parts at a time their factors through shared memory and four numbers of
-// each part a thread and load.  All in the order of the parts.
-constexpr int CHUNK = 32;
+// columns' references and sums by every warp, then a chunk of parts at a time their factors through shared memory and four numbers
+// of each part a thread and load.  All in the order of the parts.  The first parts' numbers are asked for together with the
+// references, and the first chunk's factors come from registers: one round trip instead of three.
 template <typename T, int NT>
 __device__ __forceinline__ void join_parts(const Out out, const float* first, const float* rest, int n, float* s_out,
                                            float (*s_fac)[8 * NT], int q_start, int col0, int cols, int kvh) {
   using L = Layout<T, NT>;
-  constexpr int COLS = L::COLS, FOURS = (COLS * HD / 4 + 127) / 128;
+  constexpr int COLS = L::COLS, FOURS = (COLS * HD / 4 + 127) / 128, APART = 32 / COLS, CHUNK = 8 * APART;
+  constexpr int AHEAD = FOURS == 1 ? 6 : 2;
   constexpr bool EVEN = COLS * HD / 4 % 128 == 0;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto part = [&](int i) { return i == 0 ? first : rest + (long long)i * 2 * L::PART; };
-  // a lane its column (lane % COLS), every (32 / COLS)-th part
-  float top = LOWEST, topM = LOWEST, sum = 0.f;
+  float4 ahead[AHEAD][FOURS];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+    for (int f = 0; f < FOURS; f++)
+      ahead[i][f] = __ldcg(reinterpret_cast<const float4*>(part(min(i, n - 1))) + (EVEN ? threadIdx.x + 128 * f : min(threadIdx.x + 128 * f, COLS * HD / 4 - 1)));
+  // a lane its column (lane % COLS), every APART-th part
+  float top = LOWEST, topM = LOWEST, sum = 0.f, held[8];
+  {
+    float m[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int i = lane / COLS + k * APART;
+      const float* p = part(min(i, n - 1)) + COLS * HD + lane % COLS;
+      held[k] = __ldcg(p), m[k] = __ldcg(p + COLS), l[k] = __ldcg(p + 2 * COLS);
+      if (i >= n) held[k] = m[k] = LOWEST, l[k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) topM = fmaxf(topM, held[k]), top = fmaxf(top, m[k]);
+#pragma unroll
+    for (int k = 0; k < 8; k++) sum += l[k] * ex2(m[k] - top);
+  }
 #pragma unroll 4
-  for (int i = lane / COLS; i < n; i += 32 / COLS) {
+  for (int i = lane / COLS + CHUNK; i < n; i += APART) {
     const float* p = part(i) + COLS * HD + lane % COLS;
     const float M = __ldcg(p), m = __ldcg(p + COLS), l = __ldcg(p + 2 * COLS), m2 = fmaxf(top, m);
     topM = fmaxf(topM, M);
@@ -296,26 +317,37 @@ __device__ __forceinline__ void join_parts(const Out out, const float* first, co
   sum *= ex2(mine - top);
 #pragma unroll
   for (int d = COLS; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    if (k % 4 == warp) s_fac[lane / COLS + k * APART][lane % COLS] = ex2(held[k] - topM);
+  asm volatile("bar.sync 1, 128;" ::: "memory");
   float4 acc[FOURS];
 #pragma unroll
   for (int f = 0; f < FOURS; f++) acc[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int i, int f, const float4& x) {
+    const float4 y = *reinterpret_cast<const float4*>(&s_fac[i][(threadIdx.x + 128 * f) * 4 % COLS]);
+    acc[f].x = fmaf(x.x, y.x, acc[f].x), acc[f].y = fmaf(x.y, y.y, acc[f].y);
+    acc[f].z = fmaf(x.z, y.z, acc[f].z), acc[f].w = fmaf(x.w, y.w, acc[f].w);
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++)
+    if (i < n) {
+#pragma unroll
+      for (int f = 0; f < FOURS; f++) add(i, f, ahead[i][f]);
+    }
   for (int i0 = 0; i0 < n; i0 += CHUNK) {
     const int k = min(CHUNK, n - i0);
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    for (int i = threadIdx.x / COLS; i < k; i += 128 / COLS) s_fac[i][lane % COLS] = ex2(__ldcg(part(i0 + i) + COLS * HD + lane % COLS) - topM);
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (i0 > 0) {
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int i = threadIdx.x / COLS; i < k; i += 128 / COLS) s_fac[i][lane % COLS] = ex2(__ldcg(part(i0 + i) + COLS * HD + lane % COLS) - topM);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
 #pragma unroll 8
-    for (int i = 0; i < k; i++) {
+    for (int i = i0 > 0 ? 0 : AHEAD; i < k; i++) {
       const float4* p = reinterpret_cast<const float4*>(part(i0 + i));
 #pragma unroll
-      for (int f = 0; f < FOURS; f++) {
-        const int at = threadIdx.x + 128 * f;
-        if (EVEN || at < COLS * HD / 4) {
-          const float4 x = __ldcg(p + at), y = *reinterpret_cast<const float4*>(&s_fac[i][at * 4 % COLS]);
-          acc[f].x = fmaf(x.x, y.x, acc[f].x), acc[f].y = fmaf(x.y, y.y, acc[f].y);
-          acc[f].z = fmaf(x.z, y.z, acc[f].z), acc[f].w = fmaf(x.w, y.w, acc[f].w);
-        }
-      }
+      for (int f = 0; f < FOURS; f++)
+        if (EVEN || threadIdx.x + 128 * f < COLS * HD / 4) add(i, f, __ldcg(p + threadIdx.x + 128 * f));
     }
   }
 #pragma unroll
