@@ -44,6 +44,11 @@ class Int8PagedAttention(PagedAttention):
     def _project(self, ctx, h, w, codes):
         return ops.linear(h, w) if codes is None else int8.linear_int8(h, *codes, ctx.status)
 
+    def _project_out(self, ctx, attn):
+        if self.o_codes is None and ops.can_use_few_rows(attn, self.w_o, ops.ATTN_FEW_ROWS_MAX):
+            return ops.linear_few_rows(attn, self.w_o, ctx.status)  # (slices, which the norm behind adds up)
+        return self._project(ctx, attn, self.w_o, self.o_codes)
+
     def forward(self, ctx, h, cache, out_rows=None):
         hd, nh, nkv = self.head_dim, self.n_heads, self.n_kv_heads
         tables = ctx.tables[cache.group]
@@ -52,7 +57,7 @@ class Int8PagedAttention(PagedAttention):
         if not self.int8_cache:
             ops.rope_kv_write(qkv, ctx.positions, ctx.token_seq, tables.indptr, tables.page_ids, self.inv_freq, cache.k, cache.v,
                               nh, nkv, hd, rot, cache.page_size, cache.writable, ctx.status)
-            return self._project(ctx, self.attend(ctx, qkv, cache, out_rows), self.w_o, self.o_codes)
+            return self._project_out(ctx, self.attend(ctx, qkv, cache, out_rows))
         int8.rope_kv8_write(qkv, ctx.positions, ctx.token_seq, tables.indptr, tables.page_ids, self.inv_freq, cache.k, cache.v,
                             cache.k_scale, cache.v_scale, nh, nkv, hd, rot, cache.page_size, cache.writable, ctx.status)
         attn = torch.empty((h.shape[0], nh * hd), dtype=h.dtype, device=h.device)
@@ -63,7 +68,7 @@ class Int8PagedAttention(PagedAttention):
             wanted = torch.empty((out_rows.numel(), nh * hd), dtype=h.dtype, device=h.device)
             ops.gather_rows(attn, out_rows, wanted)
             attn = wanted
-        return self._project(ctx, attn, self.w_o, self.o_codes)
+        return self._project_out(ctx, attn)
 
     @staticmethod
     def _bounds(ctx, tables, page_size: int) -> dict:
