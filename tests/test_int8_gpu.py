@@ -272,3 +272,25 @@ def test_products_in_a_graph():
         a = int8.linear_int8(x, w, t, st)
         assert torch.equal(y, a) and torch.equal(z, int8.linear_int8(a, w[:, :512], t, st))
     assert int(st) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_numbers_next_to_a_half_code(dtype):
+    """Quotients within a few units of a half integer, on either side and on it, under scales of every size."""
+    from tokasaurus_b200.kernels import int8
+
+    g = np.random.default_rng(5)
+    rows_ = []
+    for i in range(300):
+        top = np.float32(np.exp(g.uniform(-85, 85)))
+        if dtype == BF:
+            top = np.float32(torch.tensor(float(top)).to(BF).float())
+        s = top * np.float32(1 / 127)
+        x = ((g.integers(-126, 127, 512) + 0.5) * np.float64(s)).astype(np.float32)
+        x = (x.view(np.int32) + g.integers(-2, 3, 512).astype(np.int32)).view(np.float32)
+        x[7] = top
+        rows_.append(x)
+    x = torch.from_numpy(np.stack(rows_)).to(dtype).to(DEV)
+    got, scale = int8.quantise_rows(x)
+    want, want_scale = plain_quantise(x)
+    assert torch.equal(scale.cpu(), want_scale) and torch.equal(got.cpu(), want)
