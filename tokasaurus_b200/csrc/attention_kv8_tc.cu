@@ -15,6 +15,10 @@
 // The exponentials of a row use a reference that stays put while its scores stay below it + 4 (log2); when a row tops that, its
 // warp scales its rows of O.  Queries are brought to [1, 2) by a power of two a row; in float32 steps Q and P go in as two halves
 // each (22 bits).  Every wait is bounded (TKB_STATUS_WAIT_TIMEOUT).
+//
+// What bounds it: each unit's chain S - softmax - P - O, two of which a block has (one works on scores while the other's products run);
+// the tensor pipe works in 12 % of the cycles, the schedulers issue in 39 %.  2,048 tokens, 32 heads on 8 of 64 58.5 us (293 TFLOP/s),
+// of 128 87 (395); 512 behind 2,048, heads of 64, 37; 8,192 646 (425).
 #include "tcgen05.cuh"
 #include "per_device.h"
 #include <cuda_fp16.h>

@@ -20,8 +20,9 @@ namespace {
 // A block takes a kv head and a window of `per` tokens and writes the segments that lead in it: four warps a side, each every fourth
 // row of a chunk of 16.  A warp's numbers of a chunk are asked for together and stay in registers between the search for the
 // largest and the codes (segments of several chunks are read twice).  A block for every token behind these rotates its q heads.
-// What bounds it: the latency of the lookups and of the rows in small steps, the rows' bytes in long ones.  (A warp a head and
-// side with all 16 rows: 8,000 prompt tokens of 8 kv heads of 128 37 us.)
+// What bounds it: the latency of the lookups and of the rows in small steps (64 single tokens 4 us), instructions in long ones (8,000
+// prompt tokens of 8 kv heads of 128 30 us, issue slots 70 % full, 33 MB read and 16 MB written).  (A warp a head and side with
+// all 16 rows: 37 us.)
 constexpr int SIDE_WARPS = 4, W_THREADS = 2 * SIDE_WARPS * 32, CHUNK = 16;
 
 // Four numbers as they lie in memory, and as float32: apart, so that many loads can be on their way.
@@ -246,6 +247,7 @@ rope_kv8_write_kernel(T* __restrict__ qkv, const int* __restrict__ positions, co
   }
 }
 
+// A block a page, kv head and side.  Bounded by the bytes it writes: 4,032 blocks of 16 x 128 numbers a side 15 us, 83 MB at 5.4 TB/s.
 __global__ void __launch_bounds__(256)
 read_kv8_kernel(const int8_t* __restrict__ kcache, const int8_t* __restrict__ vcache, const float* __restrict__ k_scale,
                 const float* __restrict__ v_scale, const int* __restrict__ pages, float* __restrict__ k_out, float* __restrict__ v_out,

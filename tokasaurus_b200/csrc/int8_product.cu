@@ -7,8 +7,9 @@
 // w, t: an output channel's codes and scale.  The sum is a 32-bit integer, exact for K up to 132,103 (127 * 128 * K < 2^31):
 // however K is cut and in whichever order its parts are added, a token's result has the same bits.
 //
-// Both products run on the fifth-generation tensor cores (tcgen05.mma kind::i8, 32-bit integer accumulators in tensor
-// memory), fed by TMA in boxes of 128 codes (one 128-byte swizzle row) a row.  Every wait on an mbarrier is bounded: after
+// Three products, which give the same bits.  Two run on the fifth-generation tensor cores (tcgen05.mma kind::i8, 32-bit integer
+// accumulators in tensor memory), fed by TMA in boxes of 128 codes (one 128-byte swizzle row) a row: tiles of many tokens, and weights
+// streamed past few tokens.  The third takes up to 8 tokens as numbers, in one launch.  Every wait on an mbarrier is bounded: after
 // the limit the block sets TKB_STATUS_WAIT_TIMEOUT, stops waiting, frees its tensor memory and returns.
 #include "tcgen05.cuh"
 #include "int8.cuh"
@@ -21,6 +22,9 @@ namespace {
 // A block a row.  A thread's numbers (up to CHUNKS times eight, as they were loaded) stay in registers between the search for
 // the largest and the codes; what a row has beyond that is read again.  WIDE: rows start on 16-byte boundaries and are
 // read and written eight numbers at a time (their last few one by one).
+// Bounded by latency up to some hundred rows (64 rows of 2,048 bfloat16 numbers 2.1 us), then by instructions, about 30 a number
+// (2,048 rows of 8,192 13.3 us, of 50 MB at 3.8 TB/s; 8,192 of 2,048 14.9).  One to eight warps a row that fetch their next row
+// meanwhile took 20 us for either: fewer warps hide less of the way from numbers to codes.
 constexpr int CHUNKS = 4;
 
 template <typename T, bool WIDE> struct Eight;
@@ -176,6 +180,10 @@ __device__ __forceinline__ void store8(float* dst, const float (&y)[8], bool who
 // A block computes 128-token x BN-channel tiles, one after the other (persistent).  Warp 0: one lane issues the TMA loads into a
 // ring of stages; warp 1: tensor memory, one lane issues the MMAs; warps 2-5: a tile's accumulator from tensor memory, scaled
 // (gated: silu(gate) * up) and stored while the next tile's MMAs fill the other accumulator.
+// Bounded by power: 2,048 tokens x 2,048 x 16,384 gated 52 us (2.6e15 operations a second), 4,096 x 4,096 x 28,672 gated 321 us (3.0e15)
+// and 378 in a long run; of zeros the latter takes 283.  The library's product of the same codes, without scales and gate, takes 310 and
+// 241.  Pairs of SMs on one 256 x 256 tile, which read a third less from shared memory, gained 1 to 5 % on the largest and lost 4
+// to 8 % on up to 2,048 tokens.
 constexpr int BM = 128;
 
 template <int BN> struct Cfg {
@@ -345,10 +353,13 @@ int launch_many(const void* a, long long lda, const float* a_scale, const void* 
 
 // ------------------------------------------------------------------------------------------------ few tokens
 // The CHANNELS are the 128-row side of the instruction and the tokens its 16 to 128 columns, so that the weights stream at memory
-// speed whatever the token count.  A block owns 128 channels and one part of K; the parts of one tile form a CLUSTER, whose
-// blocks hand their 32-bit sums to one another through shared memory (each sums the tokens that are its own, in integers:
-// the order does not matter), scale them and store them.  With programmatic dependent launch the weights of the first stages
-// are on their way while the tokens are still being brought to codes.
+// speed whatever the token count.  A block owns 128 channels, a tile of tokens and one part of K; the parts of one tile form a
+// CLUSTER, whose blocks hand their 32-bit sums to one another through shared memory (each sums the tokens that are its own, in
+// integers: the order does not matter), scale them and store them.  With programmatic dependent launch the weights of the first
+// stages are on their way while the tokens are still being brought to codes.
+// Bounded by the weights' bytes where they are many (8 tokens x 2,048 x 128,256: 47 us, 5.6 TB/s), else by the way there and back: tensor
+// memory and barriers, the first box, the exchange of the sums (8 tokens x 2,048 x 2,048 4.2 us; 64 x 4,096 x 6,144 10.7, 2.3 TB/s;
+// 333 x 1,001 x 509 4.8).
 constexpr int BC = 128;                // channels a block
 constexpr int W8_BYTES = BC * BK8;     // 16 KiB
 
@@ -623,9 +634,13 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
 //     mma.sync 16 channels x 8 tokens x 32 in 8-bit integers,
 // a lane 16 codes of two channels a load, which serve two instructions (the tokens' codes are read in the same order of K, so that
 // neither side is rearranged).  Slices are added up in shared memory.  Gate and up rows of a group of 16 meet in one warp.
+// Against quantise_rows and the product above: 1 token x 2,048 x 2,048 6.0 -> 4.3 us, 8,192 x 2,048 10.0 -> 7.0, 2,048 x 16,384 gated
+// 10.2 -> 9.6 (3.5 TB/s; what it waits for is the tokens' way to codes, then loads: 64 KiB an SM are on their way).  Beyond
+// ROWS_NUMBERS every block's work on the tokens costs more than the launch it saves (8 tokens of 2,048: 0.06 ms more a step of 16
+// layers), and beyond ROWS_WEIGHTS TMA keeps more bytes on their way (1 x 4,096 x 28,672 gated 24.6 against 28 us).
 constexpr int ROWS_WARPS = 16, ROWS_TOKENS = 8, ROWS_STEPS = 4;  // steps of 64 codes a turn
 constexpr int ROWS_NUMBERS = 8192;                              // of all tokens, at most
-constexpr long long ROWS_WEIGHTS = 1ll << 25;
+constexpr long long ROWS_WEIGHTS = 1ll << 25;  // codes, at most
 
 __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
   uint4 v;
@@ -832,19 +847,15 @@ TKB_EXPORT int tkb_quantise_rows(const void* x, long long ldx, int f32, void* co
   return f32 ? quantise<float>(x, ldx, codes, ldc, (float*)scale, M, K, st) : quantise<bf16>(x, ldx, codes, ldc, (float*)scale, M, K, st);
 }
 
-// Bytes of scratch that tkb_linear_int8 wants with the same arguments: M float32 (padded to 16 bytes), then M rows of K codes padded
-// to 16 bytes each, or none where the product makes the codes itself.
-TKB_EXPORT long long tkb_linear_int8_scratch(const void* x, long long ldx, int x_f32, int M, int N, int K) {
-  return M <= 0 || K <= 0 || takes_rows(x, ldx, x_f32, M, N, K) ? 0 : ((long long)M * 4 + 15) / 16 * 16 + M * (((long long)K + 15) / 16 * 16);
-}
-
-// Both in one call.
+// Both in one call.  scratch: room for M float32 (padded to 16 bytes), then M rows of K codes padded to 16 bytes each; without any
+// (null) the product makes the codes itself, of as many tokens, numbers and weights as it takes.
 TKB_EXPORT int tkb_linear_int8(const void* x, long long ldx, int x_f32, const void* w, long long ldw, const float* w_scale, void* out,
                                long long ldo, int f32, void* scratch, int M, int N, int K, int gated, int* status, void* st) {
   if (M <= 0 || N <= 0) return 0;
   int rc = check(w, ldw, K, N, gated);
   if (rc) return rc;
-  if (takes_rows(x, ldx, x_f32, M, N, K)) {
+  if (!scratch) {
+    if (!takes_rows(x, ldx, x_f32, M, N, K)) return -2;
 #define TKB_ARGS x, ldx, w, ldw, w_scale, out, ldo, M, N, K, (cudaStream_t)st
     if (gated)
       return x_f32 ? f32 ? launch_rows<true, float, float>(TKB_ARGS) : launch_rows<true, float, bf16>(TKB_ARGS)

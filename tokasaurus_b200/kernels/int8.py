@@ -18,6 +18,8 @@ from tokasaurus_b200.kernels import ops
 from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, _need_cuda, _stream, _suffix, check_head_dim
 
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
+# Tokens, their numbers and weights up to which a product takes tokens as they are, in one launch (csrc/int8_product.cu has the measures).
+ROWS_TOKENS, ROWS_NUMBERS, ROWS_WEIGHTS = 8, 8192, 1 << 25
 KV8_TC_MAX_DIM = 128  # head sizes whose scores and output fit tensor memory for two units
 
 
@@ -30,7 +32,6 @@ _ARGS = {
     "tkb_attn_kv8": (_P, _L, _P, _L, _I) + (_P,) * 10 + (_I,) * 7 + (_F, _I, _I, _I, _P, _P),
     "tkb_attn_kv8_tc": (_P, _L, _P, _L, _I) + (_P,) * 9 + (_I,) * 6 + (_F, _I, _I, _P, _P),
     "tkb_attn_kv8_scratch": (_I,) * 6,
-    "tkb_linear_int8_scratch": (_P, _L, _I, _I, _I, _I),
     "tkb_linear_int8": (_P, _L, _I, _P, _L, _P, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P),
 }
 _functions: dict = {}
@@ -138,12 +139,14 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, status:
     cols = N // 2 if gated else N
     # (new_empty without a type costs a quarter less on the host than torch.empty)
     out = x.new_empty((M, cols)) if out_dtype == x_dtype else x.new_empty((M, cols), dtype=out_dtype)
-    need = _entry("int8_product.cu", "tkb_linear_int8_scratch")(x.data_ptr(), x.stride(0), x_f32, M, N, K)
-    scratch = w.new_empty((need,)) if need else None
+    x_ptr, x_stride = x.data_ptr(), x.stride(0)
+    rows = (M <= ROWS_TOKENS and M * K <= ROWS_NUMBERS and N * K <= ROWS_WEIGHTS and K % 16 == 0 and x_ptr % 16 == 0
+            and (M == 1 or x_stride * (4 if x_f32 else 2) % 16 == 0))
+    scratch = None if rows else w.new_empty(((M * 4 + 15) // 16 * 16 + M * ((K + 15) // 16 * 16),))
     _check(_entry("int8_product.cu", "tkb_linear_int8")(
-        x.data_ptr(), x.stride(0), x_f32, w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols, f32,
-        scratch.data_ptr() if need else None, M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
-    if need:
+        x_ptr, x_stride, x_f32, w.data_ptr(), w_stride, w_scale.data_ptr(), out.data_ptr(), cols, f32,
+        None if rows else scratch.data_ptr(), M, N, K, 1 if gated else 0, status.data_ptr(), _stream()), what)
+    if not rows:
         ops.LAUNCHES += 1  # two kernels
     return out
 
