@@ -226,8 +226,7 @@ def read_kv8(kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, 
     pool = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
     _check_i32(what, pages)
     n = pages.numel()
-    out = torch.empty((2, n, n_kv, ps, hd), dtype=torch.float32, device=kcache.device)
-    k, v = out.unbind(0)
+    k, v = k_scale.new_empty((n, n_kv, ps, hd)), k_scale.new_empty((n, n_kv, ps, hd))
     _check(_entry("cache8.cu", "tkb_read_kv8")(
         kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, n_kv, ps * hd,
         pool, status.data_ptr(), _stream()), what)
