@@ -17,13 +17,14 @@ using namespace tkb;
 
 namespace {
 
-// A block takes a kv head and a window of `per` tokens and writes the segments that lead in it: four warps a side, each every fourth
-// row of a chunk of 16.  A warp's numbers of a chunk are asked for together and stay in registers between the search for the
-// largest and the codes (segments of several chunks are read twice).  A block for every token behind these rotates its q heads.
+// A block takes a kv head and a window of `per` tokens and writes the segments that lead in it: SIDE_WARPS warps a side, each every
+// SIDE_WARPS-th row of a chunk of 16.  A warp's numbers of a chunk are asked for together and stay in registers between the search for
+// the largest and the codes (segments of several chunks are read twice).  A block for every token behind these rotates its q heads.
 // What bounds it: the latency of the lookups and of the rows in small steps (64 single tokens 4 us), instructions in long ones (8,000
-// prompt tokens of 8 kv heads of 128 30 us, issue slots 70 % full, 33 MB read and 16 MB written).  (A warp a head and side with
-// all 16 rows: 37 us.)
-constexpr int SIDE_WARPS = 4, W_THREADS = 2 * SIDE_WARPS * 32, CHUNK = 16;
+// prompt tokens of 8 kv heads of 128 25 us; 33 MB read and 16 MB written).  Half the instructions are a segment's, whatever its
+// numbers are, in every warp: two warps a side in long steps (four: 29 us; 512 single tokens of heads of 64 14.4 us, four: 19.0), four in
+// short ones, whose rows come sooner (8 single tokens of heads of 128 3.7 us, two: 4.7; 600 in one portion 9.2, two: 9.9).
+constexpr int CHUNK = 16;
 
 // Four numbers as they lie in memory, and as float32: apart, so that many loads can be on their way.
 __device__ __forceinline__ float4 raw_four(const float* p) { return *reinterpret_cast<const float4*>(p); }
@@ -62,14 +63,20 @@ __device__ __forceinline__ float4 rotated_each(const T* x, int d, int half, cons
   }
   return make_float4(r[0], r[1], r[2], r[3]);
 }
-template <typename T, int WORDS, bool ROT>
-__global__ void __launch_bounds__(W_THREADS, WORDS > 4 ? 2 : ROT ? 4 : 5)
+template <int SIDE_WARPS, int WORDS, bool ROT> constexpr int write_blocks() {  // an SM
+  if (SIDE_WARPS == 4) return WORDS > 4 ? 2 : ROT ? 4 : 5;
+  return WORDS > 8 ? 3 : WORDS > 4 ? 6 : ROT ? 7 : 8;
+}
+// WORDS: of four numbers, of a chunk a lane.
+template <typename T, int SIDE_WARPS, int WORDS, bool ROT>
+__global__ void __launch_bounds__(2 * SIDE_WARPS * 32, (write_blocks<SIDE_WARPS, WORDS, ROT>()))
 rope_kv8_write_kernel(T* __restrict__ qkv, const int* __restrict__ positions, const int* __restrict__ token_seq,
                       const int* __restrict__ page_indptr, const int* __restrict__ page_ids, const float* __restrict__ inv_freq,
                       int8_t* __restrict__ kcache, int8_t* __restrict__ vcache, float* __restrict__ k_scale,
                       float* __restrict__ v_scale, int tokens, int per, int nh, int nkv, int hd, int rot, unsigned word_mul, int ps,
                       int ps_shift, int num_pages, int writers, int* __restrict__ status) {
   extern __shared__ __align__(16) float cs[];  // [CHUNK][rot]
+  constexpr int W_THREADS = 2 * SIDE_WARPS * 32;
   __shared__ unsigned s_top[2 * SIDE_WARPS];
   trigger_dependents();
   grid_dependency_wait();
@@ -286,21 +293,24 @@ TKB_EXPORT int tkb_rope_kv8_write(void* qkv, int f32, const int* positions, cons
   const int ps_shift = (ps & (ps - 1)) == 0 ? 31 - __builtin_clz(ps) : -1;
   const size_t smem = (size_t)CHUNK * rot * 4;
   const unsigned word_mul = hd > 4 ? 0xffffffffu / (unsigned)(hd / 4) + 1u : 0u;
-  auto go = [&](auto* rows, auto most, auto turns) {
+  auto go = [&](auto* rows, auto warps, auto most, auto turns) {
     using T = std::remove_pointer_t<decltype(rows)>;
-    constexpr auto kernel = rope_kv8_write_kernel<T, decltype(most)::value, decltype(turns)::value>;
-    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(W_THREADS), smem, (cudaStream_t)st_, rows, positions, token_seq, page_indptr,
-                      page_ids, inv_freq, (int8_t*)kcache, (int8_t*)vcache, k_scale, v_scale, tokens, per, nh, nkv, hd, rot, word_mul, ps, ps_shift,
-                      num_pages, (int)writers, status);
+    constexpr auto kernel = rope_kv8_write_kernel<T, decltype(warps)::value, decltype(most)::value, decltype(turns)::value>;
+    return launch_pdl(kernel, dim3((unsigned)blocks), dim3(2 * decltype(warps)::value * 32), smem, (cudaStream_t)st_, rows, positions, token_seq,
+                      page_indptr, page_ids, inv_freq, (int8_t*)kcache, (int8_t*)vcache, k_scale, v_scale, tokens, per, nh, nkv, hd, rot, word_mul,
+                      ps, ps_shift, num_pages, (int)writers, status);
   };
-  auto by_type = [&](auto most) {
-    if (rot == 0) return f32 ? go((float*)qkv, most, std::false_type()) : go((__nv_bfloat16*)qkv, most, std::false_type());
-    return f32 ? go((float*)qkv, most, std::true_type()) : go((__nv_bfloat16*)qkv, most, std::true_type());
+  auto by_type = [&](auto warps, auto most) {
+    if (rot == 0) return f32 ? go((float*)qkv, warps, most, std::false_type()) : go((__nv_bfloat16*)qkv, warps, most, std::false_type());
+    return f32 ? go((float*)qkv, warps, most, std::true_type()) : go((__nv_bfloat16*)qkv, warps, most, std::true_type());
   };
-  // words of four rows that a lane has
-  if (hd <= 64) return by_type(std::integral_constant<int, 2>());
-  if (hd <= 128) return by_type(std::integral_constant<int, 4>());
-  return by_type(std::integral_constant<int, 8>());
+  auto by_size = [&](auto warps) {  // words of a chunk's rows that a lane has
+    constexpr int SHARE = 4 / decltype(warps)::value;
+    if (hd <= 64) return by_type(warps, std::integral_constant<int, 2 * SHARE>());
+    if (hd <= 128) return by_type(warps, std::integral_constant<int, 4 * SHARE>());
+    return by_type(warps, std::integral_constant<int, 8 * SHARE>());
+  };
+  return tokens >= (hd <= 64 ? 512 : 2048) ? by_size(std::integral_constant<int, 2>()) : by_size(std::integral_constant<int, 4>());
 }
 
 // k_out, v_out: float32 [n, nkv, block]; block = page size * head size (a multiple of 16).
