@@ -332,29 +332,40 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
     const T* src = reinterpret_cast<const T*>(a.q) + (a.q_start[s] + token) * a.q_stride + (long long)head * HD;
     const bool wide = (((uintptr_t)src) & 15) == 0;
     unsigned top = 0;
+    uint4 row[sizeof(T) == 2 ? HD / 8 : 1];  // bfloat16: all of the row, asked for at once
+    if constexpr (sizeof(T) == 2) {
+      // (rows that are not live ask for the last that is)
+      if (wide) {
+#pragma unroll
+        for (int c = 0; c < HD / 8; c++) row[c] = *reinterpret_cast<const uint4*>(src + c * 8);
+      } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+        for (int c = 0; c < HD / 8; c++)
+          row[c] = make_uint4(h[8 * c] | (uint32_t)h[8 * c + 1] << 16, h[8 * c + 2] | (uint32_t)h[8 * c + 3] << 16,
+                              h[8 * c + 4] | (uint32_t)h[8 * c + 5] << 16, h[8 * c + 6] | (uint32_t)h[8 * c + 7] << 16);
+      }
+    }
     auto chunk = [&](int c, float (&v)[8]) {  // eight numbers
       if (!row_live) {
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = 0.f;
-      } else if (wide) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + c * 8), y = *reinterpret_cast<const float4*>(src + c * 8 + 4);
-          v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(src + c * 8);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      } else if constexpr (sizeof(T) == 2) {
+        const uint32_t w[4] = {row[c].x, row[c].y, row[c].z, row[c].w};
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            v[2 * e] = __uint_as_float(w[e] << 16);
-            v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-          }
+        for (int e = 0; e < 4; e++) {
+          v[2 * e] = __uint_as_float(w[e] << 16);
+          v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
         }
+      } else if (wide) {
+        const float4 x = *reinterpret_cast<const float4*>(src + c * 8), y = *reinterpret_cast<const float4*>(src + c * 8 + 4);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = to_float(src[c * 8 + e]);
       }
     };
-#pragma unroll 4
+#pragma unroll(sizeof(T) == 2 ? HD / 8 : 4)
     for (int c = 0; c < HD / 8; c++) {
       float v[8];
       chunk(c, v);
@@ -365,10 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
     const float down = __uint_as_float(e >= 127 ? 0x00400000u : (unsigned)(127 - e) << 23);
     row_scale = top < 0x7f800000u ? a.scale_log2 * __uint_as_float((unsigned)(127 + e) << 23) : NAN;
     unsigned char* dst = sQ + unit * PIECES * Q_BYTES + r * 128;
-#pragma unroll 4
+#pragma unroll(sizeof(T) == 2 ? HD / 8 : 4)
     for (int c = 0; c < HD / 8; c++) {
       float v[8];
-      chunk(c, v);  // (from the cache)
+      chunk(c, v);  // (float32: from the cache)
       uint32_t h[4], low[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -383,34 +394,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
     if (streams) unit_m[r] = row_scale;
     fence_proxy_async();
   }
-  // ---------------- the item's largest value scale, as a power of two
-  if (warp >= CONVERT_WARP) {
-    const int t = tid - CONVERT_WARP * 32;
-    const int page0 = (a.window > 0 ? max(0, first_pos - a.window + 1) : 0) / a.ps, page1 = last_pos / a.ps;  // pages that are seen
-    unsigned top = 0;
-    for (int p = page0 + t; p <= page1; p += 128) {
-      bool bad = false;
-      const int page = checked_page(__ldg(table + p), a.num_pages, bad);
-      if (page >= 0) {
-        const unsigned v = __float_as_uint(a.v_scale[(long long)page * a.nkv + kvh]);
-        if (v < 0x7f800000u) top = max(top, v);
-      }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) s_top[warp - CONVERT_WARP] = top;
-  }
-  tcgen05_fence_before();
-  __syncthreads();
-  tcgen05_fence_after();
-  const uint32_t tmem = tmem_slot;
-  // 2^(10 - e) with e the exponent of the largest: the scaled ones are below 2^11, a weight below 2^15
-  const int v_exp = min(max((int)(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])) >> 23) - 127, -110), 127);
+  uint32_t tmem = 0;
+  int v_exp = 0;
+  auto begin = [&]() {  // the queries and s_top are there, tensor memory is taken
+    tcgen05_fence_before();
+    asm volatile("bar.sync 0;" ::: "memory");
+    tcgen05_fence_after();
+    tmem = tmem_slot;
+    // 2^(10 - e) with e the exponent of the largest: the scaled ones are below 2^11, a weight below 2^15
+    v_exp = min(max((int)(max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3])) >> 23) - 127, -110), 127);
+  };
 
   if (warp >= CONVERT_WARP) {
     // ---------------- converters
     const int t = tid - CONVERT_WARP * 32, key = t >> 1, half = t & 1;
     constexpr int PAIRS = ATOMS * 2;  // 16 codes each: two 16-byte chunks of the tile's row
-    const float down = __uint_as_float((unsigned)(127 + 10 - v_exp) << 23);
     bool ok = true, bad = false;
     auto page_of = [&](int j) {
       const int k = k_begin + j * BKV + key;
@@ -438,8 +436,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
         }
       }
     };
-    fetch(0, page_of(0));
+    const int first_id = page_of(0);
     int next_id = page_of(1);
+    // the item's largest value scale, as a power of two
+    const int page0 = (a.window > 0 ? max(0, first_pos - a.window + 1) : 0) / a.ps, page1 = last_pos / a.ps;  // pages that are seen
+    unsigned top = 0;
+    for (int p = page0 + t; p <= page1; p += 128) {
+      bool other = false;
+      const int id = checked_page(__ldg(table + p), a.num_pages, other);
+      if (id >= 0) {
+        const unsigned v = __float_as_uint(a.v_scale[(long long)id * a.nkv + kvh]);
+        if (v < 0x7f800000u) top = max(top, v);
+      }
+    }
+    fetch(0, first_id);  // (on its way while the queries come)
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) s_top[warp - CONVERT_WARP] = top;
+    begin();
+    const float down = __uint_as_float((unsigned)(127 + 10 - v_exp) << 23);
     for (int j = 0; j < n_tiles; j++) {
       const int st = j % STAGES;
       if (j >= STAGES && !mbar_wait_idle(&empty[st], ((j / STAGES) - 1) & 1)) { ok = false; break; }
@@ -483,6 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
     report_bad_page(bad, a.status);
   } else if (warp >= MMA_WARP) {
     // ---------------- MMA: a warp a unit
+    begin();
     const int u = warp - MMA_WARP;
     if (u < live_units) {
       constexpr uint32_t idesc_qk = idesc_half(BQ, BKV);
@@ -526,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
       }
       if (!ok) failed = 1;
     }
-  } else if (unit < live_units) {
+  } else if (begin(), unit < live_units) {
     // ---------------- softmax and output: thread = row = lane of tensor memory
     const int u = unit, first = streams ? u : 0;
     const int n = (n_tiles - first + step - 1) / step;
@@ -557,10 +572,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
         top = max_nan(scale_max<true>(x, s_sk[st], lim_lo - key0, span, there.x), scale_max<true>(y, s_sk[st] + 32, lim_lo - key0 - 32, span, there.y));
       }
       top *= row_scale;
-      // (every tile's: a wait that leaves one out could take an older phase for the one it wants)
-      if (j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
       const bool moves = !(top - m <= REF_SLACK);
-      if (__any_sync(0xffffffffu, moves)) {
+      const bool scales = __any_sync(0xffffffffu, moves);
+      if (scales && j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
+      if (scales) {
         // rows of this warp move their reference: O and l of those rows are scaled to the new one
         const float m2 = moves ? max_nan(m, top) : m;
         const float alpha = fast_exp2(m - m2);
@@ -597,6 +612,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
+      // (every tile's, here where it is long over: a wait that left one out could take an older phase for the one it wants, and P
+      // arrives only when the one before has been taken)
+      if (!scales && j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
       if (lane == 0) mbar_arrive(&p_full[u]);
     }
     if (ok && n > 0) ok = mbar_wait(&o_done[u], (n - 1) & 1);
