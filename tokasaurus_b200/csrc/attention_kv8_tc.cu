@@ -17,8 +17,8 @@
 // each (22 bits).  Every wait is bounded (TKB_STATUS_WAIT_TIMEOUT).
 //
 // What bounds it: each unit's chain S - softmax - P - O, two of which a block has (one works on scores while the other's products run);
-// the tensor pipe works in 12 % of the cycles, the schedulers issue in 39 %.  2,048 tokens, 32 heads on 8 of 64 58.5 us (293 TFLOP/s),
-// of 128 87 (395); 512 behind 2,048, heads of 64, 37; 8,192 646 (425).
+// the tensor pipe works in 12 % of the cycles, the schedulers issue in 39 %.  2,048 tokens, 32 heads on 8 of 64 54.6 us (315 TFLOP/s),
+// of 128 75.8 (454); 512 behind 2,048, heads of 64, 35.8; 8,192 635 (433).
 #include "tcgen05.cuh"
 #include "per_device.h"
 #include <cuda_fp16.h>
@@ -572,10 +572,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
         top = max_nan(scale_max<true>(x, s_sk[st], lim_lo - key0, span, there.x), scale_max<true>(y, s_sk[st] + 32, lim_lo - key0 - 32, span, there.y));
       }
       top *= row_scale;
+      // (every tile's: a wait that leaves one out could take an older phase for the one it wants.  Only where the reference moves would do,
+      // with the others' behind P: 2,048 tokens of heads of 64 57.1 us against 54.6)
+      if (j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
       const bool moves = !(top - m <= REF_SLACK);
-      const bool scales = __any_sync(0xffffffffu, moves);
-      if (scales && j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
-      if (scales) {
+      if (__any_sync(0xffffffffu, moves)) {
         // rows of this warp move their reference: O and l of those rows are scaled to the new one
         const float m2 = moves ? max_nan(m, top) : m;
         const float alpha = fast_exp2(m - m2);
@@ -612,9 +613,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_kv8_tc_kernel(const Args a) {
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
-      // (every tile's, here where it is long over: a wait that left one out could take an older phase for the one it wants, and P
-      // arrives only when the one before has been taken)
-      if (!scales && j > 0 && !mbar_wait(&o_done[u], (j - 1) & 1)) { ok = false; break; }
       if (lane == 0) mbar_arrive(&p_full[u]);
     }
     if (ok && n > 0) ok = mbar_wait(&o_done[u], (n - 1) & 1);
