@@ -51,7 +51,7 @@ constexpr bool SWIZZLES = HD == 64 || HD == 128;
 constexpr int WINDOW = 64;           // pages that are looked up together; a tile has no more
 constexpr float SLACK = 8.f;
 constexpr int WHOLE_KEYS = 512;       // up to so many keys a request's items are not cut
-constexpr int OWN_TILES = 4;          // tiles by which shares of one item may be longer than even ones
+constexpr int OWN_TILES = 3;          // tiles by which shares of one item may be longer than even ones
 constexpr float LOWEST = -1e30f;  // a reference before the first key
 
 __host__ __device__ constexpr int max_nt() { return HD <= 128 ? 2 : 1; }
@@ -428,7 +428,9 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   scan();
   Shares shares{total / (int)gridDim.x, total % (int)gridDim.x};
   // Even shares hold parts of two items here and there: twice the way from queries to results, and two joins.  Where shares that start
-  // with their items, as many tiles each, are little longer, those are taken.
+  // with their items, as many tiles each, are little longer, those are taken.  Heads of 64, even and own shares: 2 requests of 8,000
+  // keys 20.5 and 16.7 us, 8 of 2,100 18.7 and 14.8, 16 of 2,100 (two tiles longer) 21.5 and 20.4, 16 of 4,000 (four) 27.6 and 31.2; of
+  // 128, 12 of 2,100 (three) 25.6 and 23.5.
   const int even = shares.each + (shares.rest > 0), own = items < (int)gridDim.x ? (total + gridDim.x - items - 1) / (gridDim.x - items) : 0x7fffffff;
   const bool one = !a.whole && own - OWN_TILES <= even;
   if (one) {
