@@ -17,6 +17,7 @@ import torch
 from tokasaurus_b200.kernels import ops
 from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, _need_cuda, _stream, _suffix, check_head_dim
 
+_INT8, _INT32, _FLOAT32 = torch.int8, torch.int32, torch.float32
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
 # Tokens, their numbers and weights up to which a product takes tokens as they are, in one launch (csrc/int8_product.cu has the measures).
 ROWS_TOKENS, ROWS_NUMBERS, ROWS_WEIGHTS = 8, 8192, 1 << 25
@@ -52,10 +53,6 @@ def _entry(source: str, name: str, head_dim: int = 0):
 
 def _is_f32(dtype: torch.dtype) -> int:
     return 1 if _suffix(dtype) == "f32" else 0
-
-
-def _stride0(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _code_rows(rows: int, k: int, device) -> torch.Tensor:
@@ -160,22 +157,22 @@ def lay_out_codes(w: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------------------------
-def _check_cache(what: str, kcache, vcache, k_scale, v_scale, n_kv_heads: int, page_size: int, head_dim: int) -> int:
-    """The number of pages."""
+def _check_cache(what: str, kcache, vcache, k_scale, v_scale, n_kv_heads: int, page_size: int, head_dim: int) -> tuple[int, tuple]:
+    """The number of pages, and where keys, values and their scales lie."""
     shape = kcache.shape
-    if not (len(shape) == 4 and kcache.dtype == vcache.dtype == torch.int8 and shape == vcache.shape and shape[1] == n_kv_heads
-            and shape[2] == page_size and shape[3] == head_dim and kcache.is_contiguous() and vcache.is_contiguous()
-            and kcache.data_ptr() % 16 == 0 and vcache.data_ptr() % 16 == 0):
+    k, v = kcache.data_ptr(), vcache.data_ptr()
+    if not (len(shape) == 4 and shape[1:] == (n_kv_heads, page_size, head_dim) and shape == vcache.shape and kcache.dtype == vcache.dtype == _INT8
+            and kcache.is_contiguous() and vcache.is_contiguous() and k % 16 == 0 and v % 16 == 0):
         raise KernelError(f"{what}: keys and values are int8 [pages, kv heads, page size, head size] each, contiguous, on a 16-byte boundary")
-    if not (k_scale.dtype == v_scale.dtype == torch.float32 and k_scale.shape == v_scale.shape == shape[:2] and k_scale.is_contiguous()
+    if not (k_scale.dtype == v_scale.dtype == _FLOAT32 and k_scale.shape == v_scale.shape == shape[:2] and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
         raise KernelError(f"{what}: scales are float32 [pages, kv heads], contiguous")
-    return shape[0]
+    return shape[0], (k, v, k_scale.data_ptr(), v_scale.data_ptr())
 
 
 def _check_i32(what: str, *tensors) -> None:
     for t in tensors:
-        if t.dtype != torch.int32 or not t.is_contiguous():
+        if t.dtype != _INT32 or not t.is_contiguous():
             raise KernelError(f"{what}: positions, request rows, lengths and page tables are int32, contiguous")
 
 
@@ -199,7 +196,7 @@ def rope_kv8_write(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.
     if not (qkv.dim() == 2 and qkv.is_contiguous() and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim and qkv.data_ptr() % 16 == 0):
         raise KernelError(f"{what}: rows [q heads | k heads | v heads] x head size, contiguous, on a 16-byte boundary")
     n = qkv.shape[0]
-    pages = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    pages, at = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
     _check_i32(what, positions, token_seq, page_indptr, page_ids)
     if positions.numel() < n or token_seq.numel() < n:
         raise KernelError(f"{what}: a position and a request a token")
@@ -210,7 +207,7 @@ def rope_kv8_write(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.
         raise KernelError(f"{what}: inv_freq must be float32 [rotary_dim/2]")
     _check(_entry("cache8.cu", "tkb_rope_kv8_write")(
         qkv.data_ptr(), f32, positions.data_ptr(), token_seq.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr(),
-        None if inv_freq is None else inv_freq.data_ptr(), kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, n_heads,
+        None if inv_freq is None else inv_freq.data_ptr(), *at, n, n_heads,
         n_kv_heads, head_dim, rotary_dim, page_size, pages, 1 if write_cache else 0, status.data_ptr(), _stream()), what)
 
 
@@ -223,12 +220,12 @@ def read_kv8(kcache: torch.Tensor, vcache: torch.Tensor, k_scale: torch.Tensor, 
     if kcache.dim() != 4 or kcache.shape[2] * kcache.shape[3] % 16:
         raise KernelError(f"{what}: the cache is int8 [pages, kv heads, page size, head size], a page's codes of a head a multiple of 16")
     _, n_kv, ps, hd = kcache.shape
-    pool = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
+    pool, at = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv, ps, hd)
     _check_i32(what, pages)
     n = pages.numel()
     k, v = k_scale.new_empty((n, n_kv, ps, hd)), k_scale.new_empty((n, n_kv, ps, hd))
     _check(_entry("cache8.cu", "tkb_read_kv8")(
-        kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, n_kv, ps * hd,
+        *at, pages.data_ptr(), k.data_ptr(), v.data_ptr(), n, n_kv, ps * hd,
         pool, status.data_ptr(), _stream()), what)
     return k, v
 
@@ -254,10 +251,11 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     if not (n_kv_heads >= 1 and n_heads >= 1 and n_heads % n_kv_heads == 0 and page_size >= 1):
         raise KernelError(f"{what}: heads in groups of a kv head")
     width = n_heads * head_dim
-    if not (q.dim() == out.dim() == 2 and q.shape[1] >= width and out.shape[1] >= width and q.stride(1) == 1 and out.stride(1) == 1
-            and out.dtype == q.dtype and out.shape[0] >= q.shape[0]):
+    q_shape, out_shape, q_strides, out_strides = q.shape, out.shape, q.stride(), out.stride()
+    if not (len(q_shape) == len(out_shape) == 2 and q_shape[1] >= width and out_shape[1] >= width and q_strides[1] == out_strides[1] == 1
+            and out.dtype == q.dtype and out_shape[0] >= q_shape[0]):
         raise KernelError(f"{what}: rows of {n_heads} heads of {head_dim} in q and, of the same type, in out")
-    pool = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
+    pool, at = _check_cache(what, kcache, vcache, k_scale, v_scale, n_kv_heads, page_size, head_dim)
     _check_i32(what, q_start, q_len, kv_len, page_indptr, page_ids)
     n = q_len.numel()
     if q_start.numel() < n or kv_len.numel() < n or page_indptr.numel() <= n:
@@ -268,7 +266,7 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
         raise KernelError(f"{what}: scores are scaled by a positive number")
     if not (max_q_len >= 0 and max_kv_len >= 0 and 0 <= single_tokens <= n and (portions is None or portions >= 0)):
         raise KernelError(f"{what}: bounds")
-    T = q.shape[0]
+    T = q_shape[0]
     if n == 0 or T == 0:
         return
     window = window or 0
@@ -276,8 +274,9 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
     singles = min(single_tokens, T)
     exact = portions is None
     portions = (n - singles if exact else min(portions, n)) if max_q_len > 1 else 0
-    common = (q.data_ptr(), _stride0(q), out.data_ptr(), _stride0(out), f32, kcache.data_ptr(), vcache.data_ptr(), k_scale.data_ptr(),
-              v_scale.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr())
+    # (a single row's stride may be anything)
+    common = (q.data_ptr(), q_strides[0] if T > 1 else width, out.data_ptr(), out_strides[0] if out_shape[0] > 1 else width, f32, *at,
+              q_start.data_ptr(), q_len.data_ptr(), kv_len.data_ptr(), page_indptr.data_ptr(), page_ids.data_ptr())
     which, tokens, requests = 3, T, n
     if head_dim <= KV8_TC_MAX_DIM:
         # portions on the tcgen05 tensor cores, single tokens with their keys cut over the GPU
@@ -288,7 +287,8 @@ def attn_kv8(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: t
         if singles == 0:
             return
         which, tokens, requests = 1, singles, singles
-    scratch = kcache.new_empty((_entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group),))
+    need = _entry("attention_kv8.cu", "tkb_attn_kv8_scratch", head_dim)(requests, singles, tokens, max_kv_len, n_kv_heads, group)
+    scratch = kcache.new_empty((need,)) if need else None
     _check(_entry("attention_kv8.cu", "tkb_attn_kv8", head_dim)(
-        *common, scratch.data_ptr(), n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window, pool, which,
+        *common, scratch.data_ptr() if need else None, n, singles, T, max_kv_len, n_heads, n_kv_heads, page_size, scale, window, pool, which,
         status.data_ptr(), _stream()), what)
