@@ -294,3 +294,22 @@ def test_numbers_next_to_a_half_code(dtype):
     got, scale = int8.quantise_rows(x)
     want, want_scale = plain_quantise(x)
     assert torch.equal(scale.cpu(), want_scale) and torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("m,k,n,gated", [(1, 2048, 49152, False), (2, 2048, 24576, True), (1, 4096, 16384, False), (3, 512, 2048, False), (8, 1024, 4096, False),
+                                         (1, 8192, 8192, False), (1, 4096, 28672, True), (5, 16, 40, False), (4, 2064, 304, True), (1, 8176, 333, False)])
+def test_few_tokens_past_matrices_of_many_shapes(m, k, n, gated):
+    """Slices and rounds of the one-launch product, and the sizes from which on it is two: the codes' exact sums either way."""
+    from tokasaurus_b200.kernels import int8
+
+    x = rows(m, k, BF, seed=m + k)
+    w, t = codes(n, k, seed=n)
+    t = t / k**0.5
+    st = status()
+    y = int8.linear_int8(x, w, t, st, gated=gated, out_dtype=F32)
+    c, s = int8.quantise_rows(x)
+    assert torch.equal(int8.product_int8(c, s, w, t, st, gated=gated, out_dtype=F32), y) and int(st) == 0
+    sums = torch.cat([(c.double() @ part.double().t()) for part in w.split(4096)], 1)
+    z = sums * s.double()[:, None] * t.double()
+    if not gated:
+        assert ((y.double() - z).abs() <= z.abs() * 3.01 * U32 + 2.0**-126).all()

@@ -637,10 +637,11 @@ int product(const void* a, long long lda, const float* a_scale, const void* w, l
 // Against quantise_rows and the product above: 1 token x 2,048 x 2,048 6.0 -> 4.3 us, 8,192 x 2,048 10.0 -> 7.0, 2,048 x 16,384 gated
 // 10.2 -> 9.6 (3.5 TB/s; what it waits for is the tokens' way to codes, then loads: 64 KiB an SM are on their way).  Beyond
 // ROWS_NUMBERS every block's work on the tokens costs more than the launch it saves (8 tokens of 2,048: 0.06 ms more a step of 16
-// layers), and beyond ROWS_WEIGHTS TMA keeps more bytes on their way (1 x 4,096 x 28,672 gated 24.6 against 28 us).
+// layers), and beyond ROWS_WEIGHTS TMA keeps more bytes on their way (2 tokens x 2,048 x 49,152, 96 Mi: 22.1
+// against 23.3 us; x 4,096 x 28,672, 112 Mi: 27.1 against 25.8).
 constexpr int ROWS_WARPS = 16, ROWS_TOKENS = 8, ROWS_STEPS = 4;  // steps of 64 codes a turn
-constexpr int ROWS_NUMBERS = 8192;                              // of all tokens, at most
-constexpr long long ROWS_WEIGHTS = 1ll << 25;  // codes, at most
+constexpr int ROWS_NUMBERS = 8192;                               // of all tokens, at most
+constexpr long long ROWS_WEIGHTS = 3ll << 25;                    // codes, at most
 
 __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
   uint4 v;
@@ -813,8 +814,16 @@ int launch_rows(const void* x, long long ldx, const void* w, long long ldw, cons
   int rc = ask({{(const void*)product_rows_kernel<GATED, X, T>, ROWS_NUMBERS + ROWS_TOKENS * 128}});
   if (rc) return rc;
   const int groups = (N + 15) / 16, blocks = groups < sm_count() ? groups : sm_count();
-  int log2_slices = 4;
-  while (log2_slices > 0 && (long long)(ROWS_WARPS >> log2_slices) * blocks < groups) log2_slices--;
+  // Slices of K: a warp's turns cost a round trip each (1.25 us, the next one's weights on their way), a round its sums and results (0.9);
+  // of equals the one with more warps at work.  (As many slices as leave one round: 1 x 2,048 x 24,576 gated 17.8 us against 13.7.)
+  const int steps = (K + 63) / 64;
+  int log2_slices = 0;
+  long long least = 1ll << 60;
+  for (int l = 0; l <= 4; l++) {
+    const long long at_once = (long long)(ROWS_WARPS >> l) * blocks, per = (steps + (1 << l) - 1) >> l, rounds = (groups + at_once - 1) / at_once;
+    const long long cost = rounds * (4 * ((per + ROWS_STEPS - 1) / ROWS_STEPS) + 3);
+    if (cost <= least) least = cost, log2_slices = l;
+  }
   const int stride = rows_stride(K);
   return launch_pdl(product_rows_kernel<GATED, X, T>, dim3(blocks), dim3(ROWS_WARPS * 32), (size_t)M * stride, st, (const X*)x, ldx, (const int8_t*)w, ldw,
                     w_scale, (T*)out, ldo, M, N, K, log2_slices, stride);

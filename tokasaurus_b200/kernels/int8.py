@@ -20,7 +20,7 @@ from tokasaurus_b200.kernels.ops import KernelError, _check, _fn, _libs, _need, 
 _INT8, _INT32, _FLOAT32 = torch.int8, torch.int32, torch.float32
 MAX_K = 132103  # longest sum of products of two codes (127 * 128 each at most) that 32 bits hold
 # Tokens, their numbers and weights up to which a product takes tokens as they are, in one launch (csrc/int8_product.cu has the measures).
-ROWS_TOKENS, ROWS_NUMBERS, ROWS_WEIGHTS = 8, 8192, 1 << 25
+ROWS_TOKENS, ROWS_NUMBERS, ROWS_WEIGHTS = 8, 8192, 3 << 25
 KV8_TC_MAX_DIM = 128  # head sizes whose scores and output fit tensor memory for two units
 
 
